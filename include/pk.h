@@ -209,6 +209,31 @@ int pk_gemm_rope(void* stream, int trans_b, int64_t M, int64_t N, int64_t K, con
                  const void* B, int64_t ldb, void* C, int64_t ldc, const float* bias, const int32_t* pos,
                  const float* cos_sin, int64_t n_pos, int n_heads, int head_dim, int inverse);
 
+/* RMS norm of every query and key head with the rotary embedding in the same pass: per head x of
+ * head_dim values, y = R(pos) (x * rsqrt(mean(x^2) + eps) * w). q is [T, Hq * head_dim] with row
+ * stride ldq, k is [T, Hkv * head_dim] with row stride ldk (two column ranges of one packed
+ * projection, or two buffers); wq and wk are the fp32 gains [head_dim] shared by all heads of their
+ * kind. The rotation is that of pk_rope (interleaved pairs, the same table, positions outside
+ * [0, n_pos) are clamped) and applies to the first rot_q / rot_k heads; with both 0, pos and cos_sin
+ * may be NULL. Norm and rotation are fp32, the result is rounded once. Outputs may be the inputs
+ * themselves (same pointer and stride: in place); any other overlap is not allowed. Any even
+ * head_dim up to 256, any strides and alignment (16-byte aligned rows take wide accesses).
+ * The backward takes the upstream gradients dqo / dko and the inputs q / k of the forward (nothing
+ * else is saved: the norm is recomputed from the row it reads anyway) and writes dq / dk, which may
+ * be dqo / dko; dwq and dwk are ACCUMULATED (+=), each may be NULL. Replaces ops::rmsnorm per head
+ * and ops::apply_rope (src/ops.cpp:426-537), which the reference's blocks call one after the
+ * other on whole rows and on one head. */
+int pk_qk_norm_rope_fwd(void* stream, int dtype, const void* q, int64_t ldq, const void* k, int64_t ldk,
+                        const float* wq, const float* wk, void* qo, int64_t ldqo, void* ko, int64_t ldko,
+                        int64_t T, int Hq, int Hkv, int head_dim, int rot_q, int rot_k, float eps,
+                        const int32_t* pos, const float* cos_sin, int64_t n_pos);
+size_t pk_qk_norm_rope_bwd_scratch_bytes(int64_t T, int Hq, int Hkv, int head_dim);
+int pk_qk_norm_rope_bwd(void* stream, int dtype, const void* dqo, int64_t lddqo, const void* dko, int64_t lddko,
+                        const void* q, int64_t ldq, const void* k, int64_t ldk, const float* wq, const float* wk,
+                        void* dq, int64_t lddq, void* dk, int64_t lddk, float* dwq, float* dwk, void* scratch,
+                        int64_t T, int Hq, int Hkv, int head_dim, int rot_q, int rot_k, float eps,
+                        const int32_t* pos, const float* cos_sin, int64_t n_pos);
+
 /* ---- activations / elementwise ---------------------------------------------
  * SwiGLU y = silu(g) * u and its backward: ops::silu + ops::mul
  * (src/ops.cpp:404-424, 76-83). GELU (tanh form, correct derivative):
@@ -328,6 +353,51 @@ int pk_sum_to_mean(void* stream, const double* sum, double denom, float* out);
 /* dst[0..n) = value (devops::fill, include/microtorch/device_cache.hpp:104). */
 int pk_fill(void* stream, int dtype, void* dst, float value, int64_t n);
 
+/* ---- preference / policy losses over rows of logits ---------------------------------
+ * The reference trains on cross entropy only (src/ops.cpp:350-376); these entries are the losses of
+ * preference and policy tuning, beside pk_cross_entropy and with its conventions (targets int32,
+ * one row per token, out-of-range targets OR PK_ERR_INDEX into *status, which may be NULL).
+ * Rows of weight 0 (prompt, padding) are left out before anything of them is looked at: their logits
+ * are not read, whatever they hold, nor is their target (-100 is usual); their outputs are 0. A word
+ * masked with -inf or the type's lowest value has probability 0. A row that counts and holds NaN or
+ * +inf, or nothing but -inf, gives NaN, as its softmax does. A row that counts and whose target
+ * is out of range reports it and gives 0 and a zero gradient. Logits may start anywhere and have any
+ * row stride >= V; every gradient is written to dlogits [R, V] (row stride ldd), which may be logits
+ * itself (then ldd == ld); any other overlap is refused.
+ *
+ * logp[i] = logits[i, t_i] - lse[i], lse[i] = log(sum_j exp(logits[i, j])), fp32. weight may be NULL
+ * (every row counts). The backward writes dlogits[i, j] = dlogp[i] * ([j == t_i] - exp(logits[i, j] - lse[i]));
+ * rows with dlogp[i] == 0 are written as zeros without their logits being read. */
+int pk_token_logprob(void* stream, int dtype, const void* logits, int64_t ld, const int32_t* targets,
+                     const float* weight, float* logp, float* lse, int64_t R, int64_t V, int32_t* status);
+int pk_token_logprob_bwd(void* stream, int dtype, const void* logits, int64_t ld, const int32_t* targets,
+                         const float* lse, const float* dlogp, void* dlogits, int64_t ldd, int64_t R, int64_t V,
+                         int32_t* status);
+/* Paired log-ratio preference loss. Token rows are grouped into 2 * n_pairs sequences by seq
+ * [2 * n_pairs + 1] (ascending offsets into the R rows; sequences 2 i and 2 i + 1 are the chosen and
+ * the rejected answer of pair i; empty ones are allowed):
+ *     z_i    = beta * (sum over chosen of w (logp - ref) - sum over rejected of w (logp - ref))
+ *     loss_i = -(1 - label_smoothing) * log sigmoid(z_i) - label_smoothing * log sigmoid(-z_i)
+ * loss[n_pairs] and margin[n_pairs] (= z; may be NULL) are written, and dlogp [R] (may be NULL) =
+ * grad_scale * d loss / d logp for every row of a sequence; rows before the first and behind the
+ * last sequence are left as they were. weight may be NULL (1) and ref_logp may be NULL (0). Rows of
+ * weight 0 are skipped. Offsets that descend or leave [0, R] set PK_ERR_INDEX in *status; that pair's
+ * loss and margin are NaN and its rows of dlogp are left as they were. Sums are fp64 in a fixed order. */
+int pk_preference_loss(void* stream, const float* logp, const float* ref_logp, const float* weight,
+                       const int32_t* seq, int64_t n_pairs, int64_t R, float beta, float label_smoothing,
+                       float grad_scale, float* loss, float* margin, float* dlogp, int32_t* status);
+/* Clipped policy loss with a KL term, its value and its gradient in ONE pass over the logits:
+ *     r = exp(logp - old_logp), u = ref_logp - logp
+ *     row_loss = w * (-min(r A, clamp(r, 1 - clip_lo, 1 + clip_hi) A) + kl_coef * (exp(u) - u - 1))
+ *     dlogits  = grad_scale * d row_loss / d logits
+ * old_logp == NULL: the rows were sampled from this very policy (r = 1, its gradient counted);
+ * ref_logp == NULL: no KL term (kl is then 0); weight == NULL: 1. logp and kl (= exp(u) - u - 1) may be
+ * NULL; dlogits == NULL: the loss alone. On a clipping bound the unclipped branch counts. */
+int pk_policy_loss(void* stream, int dtype, const void* logits, int64_t ld, const int32_t* targets,
+                   const float* old_logp, const float* ref_logp, const float* advantage, const float* weight,
+                   float clip_lo, float clip_hi, float kl_coef, float grad_scale, float* row_loss, float* logp,
+                   float* kl, void* dlogits, int64_t ldd, int64_t R, int64_t V, int32_t* status);
+
 /* ---- optimizer ---------------------------------------------------------------
  * AdamW::step (src/nn.cpp:301-321) over a flat fp32 buffer: m,v EMA, bias
  * correction c1 = 1-b1^t, c2 = 1-b2^t computed by the caller in float,
@@ -336,6 +406,48 @@ int pk_fill(void* stream, int dtype, void* dst, float value, int64_t n);
 int pk_adamw(void* stream, float* p, const float* g, float* m, float* v, int64_t n,
              float lr, float b1, float b2, float eps, float wd, float c1, float c2,
              void* p_bf16);
+/* The same step over MANY tensors in one launch, each with its own learning-rate factor and weight
+ * decay, moments in fp32 or in 8 bits (the reference decays every parameter alike and keeps fp32
+ * moments, src/nn.cpp:301-321):
+ *     m = b1 m + (1 - b1) g, v = b2 v + (1 - b2) g^2
+ *     p -= lr * lr_mult * ((m / c1) / (sqrt(v / c2) + eps) + weight_decay * p)
+ * p is fp32, g fp32 or bf16 (one type for the plan), shadow (may be NULL) receives bf16(p).
+ * state_bits = 32: m and v are fp32 [n]; the result has the bits of pk_adamw.
+ * state_bits = 8:  m and v are E4M3 codes [n] with one power-of-two scale per 32 elements, its
+ *   exponent byte (2^(byte - 127), the E8M0 form) in m_scale / v_scale [ceil(n / 32)]: m = code * 2^(byte - 127),
+ *   and v holds sqrt(v) the same way. The update itself uses the fp32 moments before they are
+ *   rounded. m is rounded to nearest; sqrt(v) is rounded up or down at random with the right mean,
+ *   because with b2 = 0.999 a step moves v by less than half a code and rounding to nearest would
+ *   freeze it; and no sqrt(v) above zero becomes zero. The random bits are a function of `seed` (pass
+ *   another one every step) and the element's number in the plan: the same call gives the same
+ *   bits. All-zero buffers are the initial state. A moment that is not finite is stored as NaN and
+ *   does not enter its block's scale.
+ * The plan is the device-side table of the tensors, made once (pk_adamw_plan_create allocates device
+ * memory; call both outside stream captures, with the GPU current that holds the tensors). Every
+ * buffer must lie on that GPU; no written buffer may overlap another one. The step itself allocates
+ * nothing and may be captured; two steps of one plan must not run at the same time. */
+typedef struct pk_adamw_tensor {
+    float* p;
+    const void* g;
+    void* m;
+    void* v;
+    uint8_t* m_scale; /* state_bits = 8 only */
+    uint8_t* v_scale;
+    void* shadow; /* bf16 [n] or NULL */
+    int64_t n;
+    float lr_mult;
+    float weight_decay;
+} pk_adamw_tensor;
+int pk_adamw_plan_create(const pk_adamw_tensor* tensors_h, int n_tensors, int g_dtype, int state_bits, void** plan_h);
+int pk_adamw_plan_destroy(void* plan_h);
+int pk_adamw_multi(void* stream, void* plan_h, float lr, float b1, float b2, float eps, float c1, float c2,
+                   uint64_t seed);
+/* 8-bit moments to fp32 and back, for checkpoints: x = code * 2^(byte - 127), and codes and scales of x
+ * with every value rounded to nearest (root = 0, the form of m) or to nearest with nothing above zero
+ * becoming zero (root = 1, the form of sqrt(v): the entries then convert v itself, squaring and taking the
+ * root). */
+int pk_adamw_moment_unpack(void* stream, const void* codes, const uint8_t* scales, float* x, int64_t n, int root);
+int pk_adamw_moment_pack(void* stream, const float* x, void* codes, uint8_t* scales, int64_t n, int root);
 /* Q8_0: blocks of 32 along a row of W[rows, cols] (cols % 32 == 0), int8 values and an
  * fp16 scale = fp16(absmax/127) (1.0 for an all-zero block); q = round-half-away(clamp(x/s)).
  * quantize_int8 / dequantize (src/quant.cpp:11-48) with block 32 and the scale stored as fp16.

@@ -140,3 +140,33 @@ def check(rc: int, what: str = "libpk call"):
     if rc != 0:
         msg = libpk().pk_last_error().decode(errors="replace")
         raise PkError(f"{what} failed with status {rc}: {msg}")
+
+
+class AdamwTensor(ctypes.Structure):
+    """pk_adamw_tensor of include/pk.h: the buffers (device addresses) and rates of one tensor."""
+    _fields_ = [("p", ctypes.c_void_p), ("g", ctypes.c_void_p), ("m", ctypes.c_void_p), ("v", ctypes.c_void_p),
+                ("m_scale", ctypes.c_void_p), ("v_scale", ctypes.c_void_p), ("shadow", ctypes.c_void_p),
+                ("n", ctypes.c_int64), ("lr_mult", ctypes.c_float), ("weight_decay", ctypes.c_float)]
+
+
+class AdamwPlan:
+    """Owner of a pk_adamw_plan_create handle: ``libpk().pk_adamw_multi(stream, plan.handle, ...)``.
+
+    The plan keeps device addresses, not the tensors behind them: whoever made them keeps them."""
+
+    def __init__(self, tensors, g_dtype: int, state_bits: int):
+        table = (AdamwTensor * max(1, len(tensors)))(*tensors)
+        self.handle = ctypes.c_void_p()
+        check(libpk().pk_adamw_plan_create(table, len(tensors), g_dtype, state_bits, ctypes.byref(self.handle)),
+              "pk_adamw_plan_create")
+
+    def close(self):
+        if getattr(self, "handle", None):
+            handle, self.handle = self.handle, None
+            check(libpk().pk_adamw_plan_destroy(handle), "pk_adamw_plan_destroy")
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:  # interpreter shutdown: the driver frees the memory with the process
+            pass
