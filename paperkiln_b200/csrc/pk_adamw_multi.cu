@@ -1,8 +1,6 @@
 // AdamW over many tensors in one launch, with fp32 or 8-bit moments.
 //
-// The plan holds one record per tensor and a map from chunk (CHUNK consecutive elements of one
-// tensor) to record, both in device memory: a CTA finds its tensor with two dependent loads
-// instead of a search. Per element the step reads p, g and both moments and writes p, both moments
+// The plan is a table of chunks in device memory, one CTA each. Per element the step reads p, g and both moments and writes p, both moments
 // and the bf16 shadow: 30 bytes with fp32 moments and gradients, 18.1 with 8-bit moments.
 //
 // 8-bit moments: E4M3 codes, one power-of-two scale per 32 elements. A scale that is a power of two
@@ -19,10 +17,15 @@ namespace {
 
 constexpr int BLOCK = 32;          // elements per scale
 constexpr int THREADS = 256;
-constexpr int CHUNK = 4096;        // elements per CTA: a multiple of 128 (one warp's vector) and of BLOCK
+constexpr int WIDE = THREADS * 4;  // elements of a CTA's pass: 4 per thread
+// Passes of a full chunk, all loaded before the first is computed. Four keep enough bytes in flight
+// for large plans; a plan that would not fill the GPU four CTAs deep that way takes chunks of one.
+constexpr int MANY = 4;
 constexpr uint64_t PLAN_MAGIC = 0x706b5f6164616d77ull;
 
-struct Rec {
+// What a CTA needs: up to passes * WIDE consecutive elements of one tensor. A record per chunk rather than per
+// tensor: the CTA's first loads are then one step from its data instead of two or a search.
+struct Chunk {
     float* p;
     const void* g;
     void* m;
@@ -30,22 +33,18 @@ struct Rec {
     uint8_t* ms;
     uint8_t* vs;
     bf16* shadow;
-    int64_t n;
-    int64_t base;         // number of the tensor's first element in the plan (tensors padded to BLOCK)
-    int64_t first_chunk;
+    int64_t number;       // number of the first element in the plan (tensors padded to BLOCK)
     float lr_mult, wd;
-    int vec;              // every buffer allows the wide accesses
-    int pad;
+    int n;
+    int vec;              // every buffer of the tensor allows the wide accesses
 };
 
 struct Plan {
     uint64_t magic;
     int device;
-    int g_dtype, bits;
+    int g_dtype, bits, passes;
     int64_t chunks;
-    void* dev;            // Rec[n], then int32[chunks]
-    const Rec* recs;
-    const int32_t* owner;
+    Chunk* dev;
 };
 
 // 32 random bits of element i under the step's key: two rounds of xor-shift and multiplication by
@@ -102,16 +101,19 @@ __device__ __forceinline__ float scaled(float x, float inv) {
 // codes from 2^-6 up are the floats whose low 20 mantissa bits are zero: adding the random bits
 // and cutting them off rounds up with the right probability. Below 2^-6 the codes are 2^-9
 // apart, as they are in [2^-6, 2^-5): there y is shifted up by 2^-6, cut, and shifted back.
+constexpr float SMALLEST_NORMAL = 0.015625f, SMALLEST = 0.001953125f;  // 2^-6, 2^-9
+__device__ __forceinline__ float cut_by_chance(float y, uint32_t rnd) {
+    return __uint_as_float((__float_as_uint(y) + (rnd & 0xfffffu)) & 0xfff00000u);
+}
 __device__ __forceinline__ float round_by_chance(float y, uint32_t rnd, bool positive) {
-    const bool low = y < 0.015625f;
-    const float z = low ? __fadd_rn(y, 0.015625f) : y;
-    float r = __uint_as_float((__float_as_uint(z) + (rnd & 0xfffffu)) & 0xfff00000u);
-    if (low) r -= 0.015625f;
-    if (positive && r == 0.0f) r = 0.001953125f;
+    const bool low = y < SMALLEST_NORMAL;
+    float r = cut_by_chance(low ? __fadd_rn(y, SMALLEST_NORMAL) : y, rnd);
+    if (low) r -= SMALLEST_NORMAL;
+    if (positive && r == 0.0f) r = SMALLEST;
     return y == y ? r : y;
 }
 __device__ __forceinline__ float round_root_nearest(float y, bool positive) {
-    return positive && y < 0.001953125f ? 0.001953125f : y;
+    return positive && y < SMALLEST ? SMALLEST : y;
 }
 
 struct Step32 {
@@ -136,6 +138,19 @@ __device__ __forceinline__ void adamw_element(float& p, float g, float& m, float
     p = __fmaf_rn(-s.lr, __fmaf_rn(s.wd, p, upd), p);
 }
 
+// sqrt.approx and __fdividef below are within 2 units of the last place; the correctly rounded forms take
+// a third of the kernel's issue slots.
+__device__ __forceinline__ float root(float x) {
+    float y;
+    asm("sqrt.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ uint32_t max_u16x2(uint32_t a, uint32_t b) {
+    uint32_t d;
+    asm("max.u16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+    return d;
+}
+
 struct Step8 {
     float lr, b1, b2, eps, ic1, isc2;  // ic1 = 1 / c1, isc2 = 1 / sqrt(c2)
     uint32_t key;
@@ -146,20 +161,28 @@ struct Step8 {
 // roundings are written out so that the wide and the narrow loop give the same bits.
 __device__ __forceinline__ void adamw8_element(float& p, float g, float& m, float& r, const Step8& s, float wd) {
     m = __fmaf_rn(s.b1, m, __fmul_rn(1.0f - s.b1, g));
-    r = __fsqrt_rn(__fmaf_rn(s.b2, __fmul_rn(r, r), __fmul_rn(__fmul_rn(1.0f - s.b2, g), g)));
-    const float upd = __fdiv_rn(__fmul_rn(m, s.ic1), __fmaf_rn(r, s.isc2, s.eps));
+    r = root(__fmaf_rn(s.b2, __fmul_rn(r, r), __fmul_rn(__fmul_rn(1.0f - s.b2, g), g)));
+    const float upd = __fdividef(__fmul_rn(m, s.ic1), __fmaf_rn(r, s.isc2, s.eps));
     p = __fmaf_rn(-s.lr, __fmaf_rn(wd, p, upd), p);
 }
 
-template <typename G> __device__ __forceinline__ void load4(const G* g, float (&f)[4]);
-template <> __device__ __forceinline__ void load4<float>(const float* g, float (&f)[4]) { Vec<float>::load(g, f); }
-template <> __device__ __forceinline__ void load4<bf16>(const bf16* g, float (&f)[4]) {
-    const uint2 w = *reinterpret_cast<const uint2*>(g);
-    f[0] = __uint_as_float(w.x << 16);
-    f[1] = __uint_as_float(w.x & 0xffff0000u);
-    f[2] = __uint_as_float(w.y << 16);
-    f[3] = __uint_as_float(w.y & 0xffff0000u);
-}
+// Four gradients as loaded, and their conversion.
+template <typename G> struct Grad4;
+template <> struct Grad4<float> {
+    uint4 raw;
+    __device__ __forceinline__ void load(const float* g) { raw = *reinterpret_cast<const uint4*>(g); }
+    __device__ __forceinline__ void get(float (&f)[4]) const { Vec<float>::unpack(raw, f); }
+};
+template <> struct Grad4<bf16> {
+    uint2 raw;
+    __device__ __forceinline__ void load(const bf16* g) { raw = *reinterpret_cast<const uint2*>(g); }
+    __device__ __forceinline__ void get(float (&f)[4]) const {
+        f[0] = __uint_as_float(raw.x << 16);
+        f[1] = __uint_as_float(raw.x & 0xffff0000u);
+        f[2] = __uint_as_float(raw.y << 16);
+        f[3] = __uint_as_float(raw.y & 0xffff0000u);
+    }
+};
 __device__ __forceinline__ void store_shadow4(bf16* s, const float (&p)[4]) {
     __nv_bfloat162 h0 = __floats2bfloat162_rn(p[0], p[1]), h1 = __floats2bfloat162_rn(p[2], p[3]);
     uint2 w;
@@ -171,124 +194,161 @@ __device__ __forceinline__ void store_shadow4(bf16* s, const float (&p)[4]) {
 // fp32 moments.
 template <typename G>
 __global__ void __launch_bounds__(THREADS)
-adamw_multi32_kernel(const Rec* __restrict__ recs, const int32_t* __restrict__ owner, Step32 s) {
-    const int64_t chunk = blockIdx.x;
-    const Rec& r = recs[owner[chunk]];
-    const int64_t at = (chunk - r.first_chunk) * CHUNK;
-    const int64_t n = min(static_cast<int64_t>(CHUNK), r.n - at);
-    s.lr *= r.lr_mult;
-    s.wd = r.wd;
-    float* p = r.p + at;
-    const G* g = static_cast<const G*>(r.g) + at;
-    float* m = static_cast<float*>(r.m) + at;
-    float* v = static_cast<float*>(r.v) + at;
-    bf16* shadow = r.shadow ? r.shadow + at : nullptr;
-    const int nv = r.vec ? static_cast<int>(n / 4) : 0;
+adamw_multi32_kernel(const Chunk* __restrict__ chunks, Step32 s) {
+    const Chunk c = chunks[blockIdx.x];
+    s.lr *= c.lr_mult;
+    s.wd = c.wd;
+    float* m = static_cast<float*>(c.m);
+    float* v = static_cast<float*>(c.v);
+    const G* g = static_cast<const G*>(c.g);
+    const int nv = c.vec ? c.n / 4 : 0;
     for (int i = threadIdx.x; i < nv; i += THREADS) {
         float pp[4], gg[4], mm[4], vv[4];
-        Vec<float>::load(p + i * 4, pp);
-        load4<G>(g + i * 4, gg);
+        Grad4<G> raw;
+        Vec<float>::load(c.p + i * 4, pp);
+        raw.load(g + i * 4);
         Vec<float>::load(m + i * 4, mm);
         Vec<float>::load(v + i * 4, vv);
+        raw.get(gg);
 #pragma unroll
         for (int e = 0; e < 4; ++e) adamw_element<true>(pp[e], gg[e], mm[e], vv[e], s);
-        Vec<float>::store(p + i * 4, pp);
+        Vec<float>::store(c.p + i * 4, pp);
         Vec<float>::store(m + i * 4, mm);
         Vec<float>::store(v + i * 4, vv);
-        if (shadow) store_shadow4(shadow + i * 4, pp);
+        if (c.shadow) store_shadow4(c.shadow + i * 4, pp);
     }
-    for (int i = nv * 4 + threadIdx.x; i < n; i += THREADS) {
-        float pi = p[i], mi = m[i], vi = v[i];
+    for (int i = nv * 4 + threadIdx.x; i < c.n; i += THREADS) {
+        float pi = c.p[i], mi = m[i], vi = v[i];
         adamw_element<false>(pi, to_f32(g[i]), mi, vi, s);
-        p[i] = pi;
+        c.p[i] = pi;
         m[i] = mi;
         v[i] = vi;
-        if (shadow) shadow[i] = __float2bfloat16_rn(pi);
+        if (c.shadow) c.shadow[i] = __float2bfloat16_rn(pi);
     }
 }
 
 // 8-bit moments. Wide part: a lane holds 4 consecutive elements, 8 lanes a block of 32; the rest (and
 // tensors whose buffers are not aligned): a lane holds one element, a warp one block.
+// A pass of the CTA moves 18 KB, so every load of the chunk is issued before the first pass is
+// computed: with one pass in flight at a time the kernel waited for memory (24 % of the copy
+// bandwidth, 27 % of the issue slots).
 template <typename G>
-__global__ void __launch_bounds__(THREADS)
-adamw_multi8_kernel(const Rec* __restrict__ recs, const int32_t* __restrict__ owner, Step8 s) {
-    const int64_t chunk = blockIdx.x;
-    const Rec& r = recs[owner[chunk]];
-    const int64_t at = (chunk - r.first_chunk) * CHUNK;
-    const int n = static_cast<int>(min(static_cast<int64_t>(CHUNK), r.n - at));
-    const float wd = r.wd;
-    s.lr *= r.lr_mult;
-    float* p = r.p + at;
-    const G* g = static_cast<const G*>(r.g) + at;
-    uint8_t* m = static_cast<uint8_t*>(r.m) + at;
-    uint8_t* v = static_cast<uint8_t*>(r.v) + at;
-    uint8_t* ms = r.ms + at / BLOCK;
-    uint8_t* vs = r.vs + at / BLOCK;
-    bf16* shadow = r.shadow ? r.shadow + at : nullptr;
-    const int64_t number = r.base + at;
-    const int wide = r.vec ? n / 128 * 128 : 0;  // whole warps only: the shuffles below take all lanes
-    const int lane = threadIdx.x & 31;
-    for (int i = threadIdx.x * 4; i < wide; i += THREADS * 4) {
-        float pp[4], gg[4], mm[4], vv[4];
-        Vec<float>::load(p + i, pp);
-        load4<G>(g + i, gg);
-        decode4(*reinterpret_cast<const uint32_t*>(m + i), pow2_of(ms[i / BLOCK]), mm);
-        decode4(*reinterpret_cast<const uint32_t*>(v + i), pow2_of(vs[i / BLOCK]), vv);
-        float am = 0.0f, av = 0.0f;
+struct Pass8 {
+    float4 p;
+    Grad4<G> g;
+    uint32_t m, v;
+    uint8_t ms, vs;
+    __device__ __forceinline__ void load(const Chunk& c, int i) {
+        p = *reinterpret_cast<const float4*>(c.p + i);
+        g.load(static_cast<const G*>(c.g) + i);
+        m = *reinterpret_cast<const uint32_t*>(static_cast<const uint8_t*>(c.m) + i);
+        v = *reinterpret_cast<const uint32_t*>(static_cast<const uint8_t*>(c.v) + i);
+        ms = c.ms[i / BLOCK];
+        vs = c.vs[i / BLOCK];
+    }
+    // Called by whole warps: lanes of a block exchange their maxima.
+    __device__ __forceinline__ void step(const Chunk& c, int i, const Step8& s) const {
+        float pp[4] = {p.x, p.y, p.z, p.w}, gg[4], mm[4], vv[4];
+        g.get(gg);
+        decode4(m, pow2_of(ms), mm);
+        decode4(v, pow2_of(vs), vv);
+        uint32_t am = 0, av = 0;  // magnitudes compared as bits: NaN and infinity are the largest
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            adamw8_element(pp[e], gg[e], mm[e], vv[e], s, wd);
-            am = fmaxf(am, finite(mm[e]) ? fabsf(mm[e]) : 0.0f);
-            av = fmaxf(av, finite(vv[e]) ? vv[e] : 0.0f);
+            adamw8_element(pp[e], gg[e], mm[e], vv[e], s, c.wd);
+            am = max(am, __float_as_uint(mm[e]) & 0x7fffffffu);
+            av = max(av, __float_as_uint(vv[e]) & 0x7fffffffu);
         }
-        Vec<float>::store(p + i, pp);
-        if (shadow) store_shadow4(shadow + i, pp);
+        Vec<float>::store(c.p + i, pp);
+        if (c.shadow) store_shadow4(c.shadow + i, pp);
+        if (__any_sync(0xffffffffu, max(am, av) >= 0x7f800000u)) {  // rare: what is not finite becomes NaN and has no say
+            am = av = 0;
 #pragma unroll
-        for (int o = 4; o > 0; o >>= 1) {
-            am = fmaxf(am, __shfl_xor_sync(0xffffffffu, am, o));
-            av = fmaxf(av, __shfl_xor_sync(0xffffffffu, av, o));
+            for (int e = 0; e < 4; ++e) {
+                if (finite(mm[e])) am = max(am, __float_as_uint(mm[e]) & 0x7fffffffu);
+                else mm[e] = __int_as_float(0x7fffffff);
+                if (finite(vv[e])) av = max(av, __float_as_uint(vv[e]) & 0x7fffffffu);
+                else vv[e] = __int_as_float(0x7fffffff);
+            }
         }
-        const uint32_t bm = scale_byte(am), bv = scale_byte(av);
+        // both maxima in one word, rounded up to their upper 16 bits: scale_byte asks for nothing below
+        uint32_t top = ((am + 0xffffu) >> 16) | ((av + 0xffffu) & 0xffff0000u);
+#pragma unroll
+        for (int o = 4; o > 0; o >>= 1) top = max_u16x2(top, __shfl_xor_sync(0xffffffffu, top, o));
+        const uint32_t bm = scale_byte(__uint_as_float(top << 16)), bv = scale_byte(__uint_as_float(top & 0xffff0000u));
         const float im = inverse_of(bm), iv = inverse_of(bv);
-        const uint32_t k0 = element_key(number + i);
+        const uint32_t k0 = element_key(c.number + i);
+        float y[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            const bool positive = vv[e] > 0.0f;
-            mm[e] = scaled(mm[e], im);
-            vv[e] = round_by_chance(scaled(vv[e], iv), mix32((k0 + e) ^ s.key), positive);
+            mm[e] *= im;
+            y[e] = vv[e] * iv;
         }
-        *reinterpret_cast<uint32_t*>(m + i) = encode4(mm);
-        *reinterpret_cast<uint32_t*>(v + i) = encode4(vv);
-        if ((lane & 7) == 0) {
-            ms[i / BLOCK] = static_cast<uint8_t>(bm);
-            vs[i / BLOCK] = static_cast<uint8_t>(bv);
+        // every value of the warp at or above the smallest normal code: the plain cut
+        if (__all_sync(0xffffffffu, fminf(fminf(y[0], y[1]), fminf(y[2], y[3])) >= SMALLEST_NORMAL && y[0] + y[1] + y[2] + y[3] < INFINITY)) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) vv[e] = cut_by_chance(y[e], mix32((k0 + e) ^ s.key));
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) vv[e] = round_by_chance(y[e], mix32((k0 + e) ^ s.key), vv[e] > 0.0f);
+        }
+        *reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(c.m) + i) = encode4(mm);
+        *reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(c.v) + i) = encode4(vv);
+        if ((threadIdx.x & 7) == 0) {
+            c.ms[i / BLOCK] = static_cast<uint8_t>(bm);
+            c.vs[i / BLOCK] = static_cast<uint8_t>(bv);
         }
     }
-    for (int b = wide / BLOCK + (threadIdx.x >> 5); b * BLOCK < n; b += THREADS / 32) {
+};
+
+template <typename G, int PASSES>
+__global__ void __launch_bounds__(THREADS, 3)
+adamw_multi8_kernel(const Chunk* __restrict__ chunks, Step8 s) {
+    const Chunk c = chunks[blockIdx.x];
+    s.lr *= c.lr_mult;
+    if (c.vec && c.n == PASSES * WIDE) {
+        Pass8<G> pass[PASSES];
+#pragma unroll
+        for (int k = 0; k < PASSES; ++k) pass[k].load(c, k * WIDE + threadIdx.x * 4);
+#pragma unroll
+        for (int k = 0; k < PASSES; ++k) pass[k].step(c, k * WIDE + threadIdx.x * 4, s);
+        return;
+    }
+    const int wide = c.vec ? c.n / 128 * 128 : 0;  // whole warps only: the shuffles take all lanes
+    for (int i = threadIdx.x * 4; i < wide; i += WIDE) {
+        Pass8<G> pass;
+        pass.load(c, i);
+        pass.step(c, i, s);
+    }
+    const int lane = threadIdx.x & 31;
+    const G* g = static_cast<const G*>(c.g);
+    uint8_t* m = static_cast<uint8_t*>(c.m);
+    uint8_t* v = static_cast<uint8_t*>(c.v);
+    for (int b = wide / BLOCK + (threadIdx.x >> 5); b * BLOCK < c.n; b += THREADS / 32) {
         const int i = b * BLOCK + lane;
-        const bool in = i < n;
+        const bool in = i < c.n;
         float pp = 0.0f, mm[4] = {}, vv[4] = {};
         if (in) {
-            pp = p[i];
-            decode4(m[i], pow2_of(ms[b]), mm);
-            decode4(v[i], pow2_of(vs[b]), vv);
-            adamw8_element(pp, to_f32(g[i]), mm[0], vv[0], s, wd);
-            p[i] = pp;
-            if (shadow) shadow[i] = __float2bfloat16_rn(pp);
+            pp = c.p[i];
+            decode4(m[i], pow2_of(c.ms[b]), mm);
+            decode4(v[i], pow2_of(c.vs[b]), vv);
+            adamw8_element(pp, to_f32(g[i]), mm[0], vv[0], s, c.wd);
+            c.p[i] = pp;
+            if (c.shadow) c.shadow[i] = __float2bfloat16_rn(pp);
         }
         const uint32_t bm = scale_byte(warp_max(in && finite(mm[0]) ? fabsf(mm[0]) : 0.0f));
         const uint32_t bv = scale_byte(warp_max(in && finite(vv[0]) ? vv[0] : 0.0f));
         if (in) {
             const bool positive = vv[0] > 0.0f;
             const float cm[4] = {scaled(mm[0], inverse_of(bm)), 0.0f, 0.0f, 0.0f};
-            const float cv[4] = {round_by_chance(scaled(vv[0], inverse_of(bv)), mix32(element_key(number + i) ^ s.key), positive),
+            const float cv[4] = {round_by_chance(scaled(vv[0], inverse_of(bv)), mix32(element_key(c.number + i) ^ s.key), positive),
                                  0.0f, 0.0f, 0.0f};
             m[i] = static_cast<uint8_t>(encode4(cm));
             v[i] = static_cast<uint8_t>(encode4(cv));
         }
         if (lane == 0) {  // after every lane has read the old scales: the shuffles above order it
-            ms[b] = static_cast<uint8_t>(bm);
-            vs[b] = static_cast<uint8_t>(bv);
+            c.ms[b] = static_cast<uint8_t>(bm);
+            c.vs[b] = static_cast<uint8_t>(bv);
         }
     }
 }
@@ -363,8 +423,10 @@ int pk_adamw_plan_create(const pk_adamw_tensor* tensors_h, int n_tensors, int g_
     int device = 0;
     PK_CHECK_CUDA(cudaGetDevice(&device));
     try {
-        std::vector<Rec> recs;
-        std::vector<int32_t> owner;
+        int64_t large = 0;
+        for (int t = 0; t < n_tensors; ++t) large += (tensors_h[t].n + MANY * WIDE - 1) / (MANY * WIDE);
+        const int passes = large >= static_cast<int64_t>(sm_count()) * 4 ? MANY : 1, CHUNK = passes * WIDE;
+        std::vector<Chunk> chunks;
         std::vector<Range> ranges;
         int64_t base = 0;
         for (int t = 0; t < n_tensors; ++t) {
@@ -381,28 +443,28 @@ int pk_adamw_plan_create(const pk_adamw_tensor* tensors_h, int n_tensors, int g_
                 const uintptr_t lo = reinterpret_cast<uintptr_t>(b.p);
                 ranges.push_back({lo, lo + b.bytes, b.written});
             }
-            Rec r{};
-            r.p = x.p;
-            r.g = x.g;
-            r.m = x.m;
-            r.v = x.v;
-            r.ms = x.m_scale;
-            r.vs = x.v_scale;
-            r.shadow = static_cast<bf16*>(x.shadow);
-            r.n = x.n;
-            r.base = base;
-            r.first_chunk = static_cast<int64_t>(owner.size());
-            r.lr_mult = x.lr_mult;
-            r.wd = x.weight_decay;
             const uintptr_t mask = 4 * ss - 1;
-            r.vec = aligned16(x.p) && (reinterpret_cast<uintptr_t>(x.g) & (4 * gs - 1)) == 0 &&
-                    (reinterpret_cast<uintptr_t>(x.m) & mask) == 0 && (reinterpret_cast<uintptr_t>(x.v) & mask) == 0 &&
-                    (reinterpret_cast<uintptr_t>(x.shadow) & 7u) == 0;
+            const int vec = aligned16(x.p) && (reinterpret_cast<uintptr_t>(x.g) & (4 * gs - 1)) == 0 &&
+                            (reinterpret_cast<uintptr_t>(x.m) & mask) == 0 && (reinterpret_cast<uintptr_t>(x.v) & mask) == 0 &&
+                            (reinterpret_cast<uintptr_t>(x.shadow) & 7u) == 0;
+            PK_REQUIRE(static_cast<int64_t>(chunks.size()) + (x.n + CHUNK - 1) / CHUNK <= 0x7fffffff, "too many elements");
+            for (int64_t at = 0; at < x.n; at += CHUNK) {
+                Chunk c{};
+                c.p = x.p + at;
+                c.g = static_cast<const char*>(x.g) + at * static_cast<int64_t>(gs);
+                c.m = static_cast<char*>(x.m) + at * static_cast<int64_t>(ss);
+                c.v = static_cast<char*>(x.v) + at * static_cast<int64_t>(ss);
+                c.ms = x.m_scale ? x.m_scale + at / BLOCK : nullptr;
+                c.vs = x.v_scale ? x.v_scale + at / BLOCK : nullptr;
+                c.shadow = x.shadow ? static_cast<bf16*>(x.shadow) + at : nullptr;
+                c.number = base + at;
+                c.lr_mult = x.lr_mult;
+                c.wd = x.weight_decay;
+                c.n = static_cast<int>(std::min<int64_t>(CHUNK, x.n - at));
+                c.vec = vec;
+                chunks.push_back(c);
+            }
             base += static_cast<int64_t>(nb) * BLOCK;
-            const int64_t chunks = (x.n + CHUNK - 1) / CHUNK;
-            PK_REQUIRE(static_cast<int64_t>(owner.size()) + chunks <= 0x7fffffff, "too many elements");
-            owner.insert(owner.end(), static_cast<size_t>(chunks), static_cast<int32_t>(recs.size()));
-            recs.push_back(r);
         }
         std::sort(ranges.begin(), ranges.end(), [](const Range& a, const Range& b) { return a.lo < b.lo; });
         uintptr_t end_any = 0, end_written = 0;  // furthest ends seen so far
@@ -416,19 +478,16 @@ int pk_adamw_plan_create(const pk_adamw_tensor* tensors_h, int n_tensors, int g_
         plan->device = device;
         plan->g_dtype = g_dtype;
         plan->bits = state_bits;
-        plan->chunks = static_cast<int64_t>(owner.size());
-        if (!recs.empty()) {
-            const size_t rb = recs.size() * sizeof(Rec), ob = owner.size() * sizeof(int32_t);
-            cudaError_t e = cudaMalloc(&plan->dev, rb + ob);
-            if (e == cudaSuccess) {
-                char* d = static_cast<char*>(plan->dev);
-                e = cudaMemcpy(d, recs.data(), rb, cudaMemcpyHostToDevice);
-                if (e == cudaSuccess) e = cudaMemcpy(d + rb, owner.data(), ob, cudaMemcpyHostToDevice);
-                plan->recs = reinterpret_cast<const Rec*>(d);
-                plan->owner = reinterpret_cast<const int32_t*>(d + rb);
-            }
+        plan->passes = passes;
+        plan->chunks = static_cast<int64_t>(chunks.size());
+        if (!chunks.empty()) {
+            const size_t bytes = chunks.size() * sizeof(Chunk);
+            void* dev = nullptr;
+            cudaError_t e = cudaMalloc(&dev, bytes);
+            if (e == cudaSuccess) e = cudaMemcpy(dev, chunks.data(), bytes, cudaMemcpyHostToDevice);
+            plan->dev = static_cast<Chunk*>(dev);
             if (e != cudaSuccess) {
-                if (plan->dev) cudaFree(plan->dev);
+                if (dev) cudaFree(dev);
                 delete plan;
                 set_error("%s: %s", __func__, cudaGetErrorString(e));
                 return PK_ERR_CUDA;
@@ -466,13 +525,14 @@ int pk_adamw_multi(void* stream, void* plan_h, float lr, float b1, float b2, flo
     cudaStream_t st = as_stream(stream);
     if (plan->bits == 32) {
         const Step32 s = {lr, b1, b2, eps, 0.0f, c1, c2};
-        if (plan->g_dtype == PK_F32) adamw_multi32_kernel<float><<<grid, THREADS, 0, st>>>(plan->recs, plan->owner, s);
-        else adamw_multi32_kernel<bf16><<<grid, THREADS, 0, st>>>(plan->recs, plan->owner, s);
+        if (plan->g_dtype == PK_F32) adamw_multi32_kernel<float><<<grid, THREADS, 0, st>>>(plan->dev, s);
+        else adamw_multi32_kernel<bf16><<<grid, THREADS, 0, st>>>(plan->dev, s);
     } else {
         const uint32_t key = mix32(static_cast<uint32_t>(seed) + 0x632BE5ABu * static_cast<uint32_t>(seed >> 32));
         const Step8 s = {lr, b1, b2, eps, static_cast<float>(1.0 / c1), static_cast<float>(1.0 / sqrt(static_cast<double>(c2))), key};
-        if (plan->g_dtype == PK_F32) adamw_multi8_kernel<float><<<grid, THREADS, 0, st>>>(plan->recs, plan->owner, s);
-        else adamw_multi8_kernel<bf16><<<grid, THREADS, 0, st>>>(plan->recs, plan->owner, s);
+        const bool f = plan->g_dtype == PK_F32;
+        if (plan->passes == MANY) (f ? adamw_multi8_kernel<float, MANY> : adamw_multi8_kernel<bf16, MANY>)<<<grid, THREADS, 0, st>>>(plan->dev, s);
+        else (f ? adamw_multi8_kernel<float, 1> : adamw_multi8_kernel<bf16, 1>)<<<grid, THREADS, 0, st>>>(plan->dev, s);
     }
     PK_LAUNCH_CHECK();
     return PK_OK;

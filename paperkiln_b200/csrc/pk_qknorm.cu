@@ -8,51 +8,125 @@
 // nothing saved by the forward and reduces once.
 //
 // Bound by memory: 2 (forward) or 3 (backward) accesses per element. A team of LANES threads owns a
-// head (16 bytes per thread), a warp walks the heads of one token and keeps the token's part of the
-// rotation table and the gains in registers; heads are taken U at a time so that U wide loads
-// per thread are in flight.
+// head, 16 bytes per thread. A warp's task is a group of heads of one kind and one token (of several
+// tokens where a token has fewer heads than the warp has teams): U heads per team, all loaded
+// before the first is computed, with the rotation table's row and the gains in registers.
 #include <algorithm>
+#include <type_traits>
 
 #include "pk_common.cuh"
+#include "pk_tc.cuh"
 
 namespace pk {
 namespace {
 
 constexpr int THREADS = 256, WARPS = THREADS / 32;
-constexpr int U = 4;  // heads per team in flight
+constexpr int U = 4;  // heads per team in flight, at most
 
-struct QkArgs {
-    const void* x[2];     // q, k: inputs of the forward
-    const void* g[2];     // upstream gradients (backward)
-    void* y[2];           // outputs: y or dx
-    int64_t ldx[2], ldg[2], ldy[2];
-    const float* w[2];
-    int heads[2], rot[2];
-    int dk;
-    float eps;
-    const int32_t* pos;
-    const float* cs;
-    int64_t n_pos, T;
-    int parts;            // warps that share a token
-    float* partial;       // backward: [blocks][2][dk] partial sums of dw, or null
+// One kind of heads (queries or keys) and how its tasks are cut.
+struct Kind {
+    const void* x;        // input of the forward
+    const void* g;        // upstream gradient (backward)
+    void* y;              // y or dx
+    int64_t ldx, ldg, ldy;
+    const float* w;
+    int heads, rot;
+    int step;             // heads side by side in a warp: a power of two, at most the warp's teams
+    int u;                // heads per team and task: U, or what divides the heads evenly
+    int rounds;           // tasks per group of tokens (teams / step tokens)
+    int64_t groups;
+    int blocks;           // backward: blocks that work on this kind
 };
 
-// N consecutive elements. Wide accesses need 16-byte aligned rows; the narrow form (N = 2, one
-// rotation pair) takes any alignment.
+struct QkArgs {
+    Kind kind[2];
+    int dk;
+    float eps;
+    const int32_t* pos;   // null: nothing is rotated
+    const float* cs;
+    int64_t n_pos, T;
+    float* partial;       // backward: [blocks][dk] partial sums of dw (queries' blocks first), or null
+};
+
+using tc::f2_add;
+using tc::f2_fma;
+using tc::f2_mul;
+using tc::f2_pack;
+using tc::f2_pack_bits;
+using tc::f2_unpack;
+
+__device__ __forceinline__ uint64_t f2_both(float v) { return f2_pack(v, v); }
+__device__ __forceinline__ float f2_sum(uint64_t v) {
+    float lo, hi;
+    f2_unpack(v, lo, hi);
+    return lo + hi;
+}
+__device__ __forceinline__ uint64_t f2_neg(uint64_t v) { return v ^ 0x8000000080000000ull; }
+
+// N consecutive elements of a head, held as even and odd ones (the two members of each rotation
+// pair) in packed fp32 pairs: the arithmetic of both kernels is two elements per instruction, which
+// matters because at copy speed an SM has 22 issue slots per bf16 element. Wide pieces are 16
+// bytes and need 16-byte aligned rows; the narrow one (N = 2) takes any alignment and leaves the
+// upper halves zero.
 template <typename T, int N> struct Piece {
-    static constexpr bool WIDE = N * sizeof(T) == 16;
-    __device__ __forceinline__ static void load(const T* p, float (&f)[N]) {
-        if constexpr (WIDE) Vec<T>::load(p, f);
-        else {
-#pragma unroll
-            for (int e = 0; e < N; ++e) f[e] = to_f32(p[e]);
+    static constexpr int P = N >= 4 ? N / 4 : 1;
+    uint64_t even[P], odd[P];
+    static __device__ __forceinline__ uint4 load_raw(const T* p) {
+        if constexpr (N * sizeof(T) == 16) return Vec<T>::load_raw(p);
+        else if constexpr (sizeof(T) == 4) return make_uint4(__float_as_uint(p[0]), __float_as_uint(p[1]), 0, 0);
+        else return make_uint4(__bfloat16_as_ushort(p[0]), __bfloat16_as_ushort(p[1]), 0, 0);
+    }
+    __device__ __forceinline__ explicit Piece(const uint4& v) {
+        if constexpr (N == 8) {
+            even[0] = f2_pack_bits(v.x << 16, v.y << 16);
+            odd[0] = f2_pack_bits(v.x & 0xffff0000u, v.y & 0xffff0000u);
+            even[1] = f2_pack_bits(v.z << 16, v.w << 16);
+            odd[1] = f2_pack_bits(v.z & 0xffff0000u, v.w & 0xffff0000u);
+        } else if constexpr (N == 4) {
+            even[0] = f2_pack_bits(v.x, v.z);
+            odd[0] = f2_pack_bits(v.y, v.w);
+        } else {
+            even[0] = f2_pack_bits(sizeof(T) == 4 ? v.x : v.x << 16, 0);
+            odd[0] = f2_pack_bits(sizeof(T) == 4 ? v.y : v.y << 16, 0);
         }
     }
-    __device__ __forceinline__ static void store(T* p, const float (&f)[N]) {
-        if constexpr (WIDE) Vec<T>::store(p, f);
-        else {
+    __device__ __forceinline__ Piece() {}
+    __device__ __forceinline__ void store(T* p) const {
+        float f[P * 4];
 #pragma unroll
-            for (int e = 0; e < N; ++e) p[e] = from_f32<T>(f[e]);
+        for (int i = 0; i < P; ++i) {
+            f2_unpack(even[i], f[4 * i], f[4 * i + 2]);
+            f2_unpack(odd[i], f[4 * i + 1], f[4 * i + 3]);
+        }
+        if constexpr (N * sizeof(T) == 16) {
+            float w[N];
+#pragma unroll
+            for (int e = 0; e < N; ++e) w[e] = f[e];
+            Vec<T>::store(p, w);
+        } else {
+            p[0] = from_f32<T>(f[0]);
+            p[1] = from_f32<T>(f[1]);
+        }
+    }
+    // fp32 values of columns c .. c + N - 1 (zeros past dk); wide pieces need 16-byte aligned tables
+    __device__ __forceinline__ void table(const float* w, int c, int dk) {
+        float f[P * 4] = {};
+        if (c < dk) {
+            if constexpr (N >= 4) {
+#pragma unroll
+                for (int i = 0; i < P; ++i) {
+                    const float4 v = *reinterpret_cast<const float4*>(w + c + 4 * i);
+                    f[4 * i] = v.x; f[4 * i + 1] = v.y; f[4 * i + 2] = v.z; f[4 * i + 3] = v.w;
+                }
+            } else {
+                f[0] = w[c];
+                f[1] = w[c + 1];
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < P; ++i) {
+            even[i] = f2_pack(f[4 * i], f[4 * i + 2]);
+            odd[i] = f2_pack(f[4 * i + 1], f[4 * i + 3]);
         }
     }
 };
@@ -65,161 +139,262 @@ __device__ __forceinline__ float team_sum(float v) {
 }
 
 // A thread holds PIECES pieces of N elements of its head: piece j covers elements
-// (j * LANES + lane) * N. Every warp works on whole warps of threads; teams past the last head and
-// lanes past dk hold zeros, so that the shuffles always take all lanes.
-template <typename T, int N, int LANES, int PIECES, bool BACK>
-__global__ void __launch_bounds__(THREADS)
-qk_norm_rope_kernel(QkArgs a) {
-    constexpr int TEAMS = 32 / LANES;
-    const int lane = threadIdx.x & 31, team = lane / LANES, tl = lane % LANES;
-    const int64_t warps = static_cast<int64_t>(gridDim.x) * WARPS;
-    const int64_t tasks = a.T * a.parts;
-    const float inv_dk = 1.0f / static_cast<float>(a.dk);
-    float dw[2][PIECES][N] = {};
-    float w[2][PIECES][N];
+// (j * LANES + lane) * N. Lanes past dk, teams past the last head or token hold zeros, so that the
+// shuffles always take all lanes.
+template <typename T, int N, int LANES, int PIECES>
+struct Place {
+    int team, tl;
+    __device__ __forceinline__ Place() : team((threadIdx.x & 31) / LANES), tl((threadIdx.x & 31) % LANES) {}
+    __device__ __forceinline__ int col(int j) const { return (j * LANES + tl) * N; }
+};
+
+__device__ __forceinline__ const float* table_row(const QkArgs& a, int64_t p) {
+    return a.cs + (p < 0 ? 0 : (p >= a.n_pos ? a.n_pos - 1 : p)) * a.dk;
+}
+
+// What a warp's task is like as a whole. The bounds, and whether a head turns, are a third of the
+// instructions of a task; where every head of the round exists, fills its lanes and turns (or none
+// does), they are left out.
+enum Form { ANY = 0, FULL_TURN = 1, FULL_PLAIN = 2 };
+template <Form F, int UU> struct Shape {};
+template <typename T, int N, int LANES, int PIECES, typename Run>
+__device__ __forceinline__ void with_shape(const QkArgs& a, const Kind& k, int first, bool tokens, Run run) {
+    const int last = first + k.step * k.u;
+    const bool full = last <= k.heads && PIECES * LANES * N == a.dk && tokens;
+    const bool turn = full && last <= k.rot, plain = full && first >= k.rot;
+    if (turn && k.u == 4) run(Shape<FULL_TURN, 4>());
+    else if (turn && k.u == 2) run(Shape<FULL_TURN, 2>());
+    else if (turn) run(Shape<FULL_TURN, 1>());
+    else if (plain && k.u == 4) run(Shape<FULL_PLAIN, 4>());
+    else run(Shape<ANY, U>());
+}
+
+template <typename T, int N, int LANES, int PIECES, Form F, int UU>
+__device__ __forceinline__ void forward_task(const QkArgs& a, const Kind& k, const Place<T, N, LANES, PIECES>& at, int64_t t, int first,
+                                             Shape<F, UU>) {
+    const int h0 = first + at.team % k.step;
+    const bool token = F != ANY || t < a.T;
+    const int heads = min(k.heads, first + k.step * k.u);  // ANY: where the round ends
+    const int hop = k.step * a.dk;
+    const T* x = static_cast<const T*>(k.x) + t * k.ldx + h0 * a.dk + at.tl * N;
+    T* y = static_cast<T*>(k.y) + t * k.ldy + h0 * a.dk + at.tl * N;
+    int64_t p = 0;
+    if (F == FULL_TURN || (F == ANY && a.pos && token)) p = a.pos[t];
+    uint4 raw[UU][PIECES];
 #pragma unroll
-    for (int r = 0; r < 2; ++r)
+    for (int u = 0; u < UU; ++u)
 #pragma unroll
-        for (int j = 0; j < PIECES; ++j)
-#pragma unroll
-            for (int e = 0; e < N; ++e) {
-                const int c = (j * LANES + tl) * N + e;
-                w[r][j][e] = c < a.dk ? a.w[r][c] : 0.0f;
-            }
-    for (int64_t task = static_cast<int64_t>(blockIdx.x) * WARPS + (threadIdx.x >> 5); task < tasks; task += warps) {
-        const int64_t t = task / a.parts;
-        const int part = static_cast<int>(task - t * a.parts);
-        float cs[PIECES][N];  // (cos, sin) of the thread's pairs; the backward turns by the negative angle
-        if (a.rot[0] + a.rot[1] > 0) {
-            int64_t p = a.pos[t];
-            p = p < 0 ? 0 : (p >= a.n_pos ? a.n_pos - 1 : p);
-            const float* row = a.cs + p * a.dk;
-#pragma unroll
-            for (int j = 0; j < PIECES; ++j)
-#pragma unroll
-                for (int e = 0; e < N; e += 2) {
-                    const int c = (j * LANES + tl) * N + e;
-                    float2 v = make_float2(1.0f, 0.0f);
-                    if (c < a.dk) v = *reinterpret_cast<const float2*>(row + c);
-                    cs[j][e] = v.x;
-                    cs[j][e + 1] = BACK ? -v.y : v.y;
-                }
+        for (int j = 0; j < PIECES; ++j) {
+            if (F == ANY) raw[u][j] = make_uint4(0, 0, 0, 0);
+            if (F != ANY || (token && h0 + u * k.step < heads && at.col(j) < a.dk))
+                raw[u][j] = Piece<T, N>::load_raw(x + u * hop + j * (LANES * N));
         }
+    // gain and angle of a pair in one: with c, s the angle's and w, w' the pair's gains,
+    // (x, x') -> inv (x wc - x' w's, x ws + x' w'c)
+    Piece<T, N> w[PIECES], wc[PIECES], ws[PIECES];  // ws.even = w s, ws.odd = -w' s
 #pragma unroll
-        for (int r = 0; r < 2; ++r) {
-            const T* x = static_cast<const T*>(a.x[r]) + t * a.ldx[r];
-            const T* g = BACK ? static_cast<const T*>(a.g[r]) + t * a.ldg[r] : nullptr;
-            T* y = static_cast<T*>(a.y[r]) + t * a.ldy[r];
-            const int H = a.heads[r];
-            for (int h0 = part * TEAMS * U; h0 < H; h0 += a.parts * TEAMS * U) {
-                float xv[U][PIECES][N], gv[BACK ? U : 1][PIECES][N];
+    for (int j = 0; j < PIECES; ++j) w[j].table(k.w, at.col(j), a.dk);
+    if (F == FULL_TURN || (F == ANY && a.pos)) {
+        const float* row = table_row(a, p);
 #pragma unroll
-                for (int u = 0; u < U; ++u) {
-                    const int h = h0 + u * TEAMS + team;
+        for (int j = 0; j < PIECES; ++j) {
+            Piece<T, N> cs;
+            cs.table(row, at.col(j), a.dk);  // cos in even, sin in odd
 #pragma unroll
-                    for (int j = 0; j < PIECES; ++j) {
-                        const int c = (j * LANES + tl) * N;
-#pragma unroll
-                        for (int e = 0; e < N; ++e) {
-                            xv[u][j][e] = 0.0f;
-                            if constexpr (BACK) gv[u][j][e] = 0.0f;
-                        }
-                        if (h < H && c < a.dk) {
-                            Piece<T, N>::load(x + h * a.dk + c, xv[u][j]);
-                            if constexpr (BACK) Piece<T, N>::load(g + h * a.dk + c, gv[u][j]);
-                        }
-                    }
-                }
-#pragma unroll
-                for (int u = 0; u < U; ++u) {
-                    const int h = h0 + u * TEAMS + team;
-                    const bool turn = h < a.rot[r];
-                    float s1 = 0.0f, s2 = 0.0f;
-#pragma unroll
-                    for (int j = 0; j < PIECES; ++j) {
-                        if constexpr (BACK) {
-                            if (turn)
-#pragma unroll
-                                for (int e = 0; e < N; e += 2) {
-                                    float o0, o1;
-                                    rope_rotate(gv[u][j][e], gv[u][j][e + 1], cs[j][e], cs[j][e + 1], o0, o1);
-                                    gv[u][j][e] = o0;
-                                    gv[u][j][e + 1] = o1;
-                                }
-                        }
-#pragma unroll
-                        for (int e = 0; e < N; ++e) {
-                            s1 += xv[u][j][e] * xv[u][j][e];
-                            if constexpr (BACK) s2 += gv[u][j][e] * w[r][j][e] * xv[u][j][e];
-                        }
-                    }
-                    s1 = team_sum<LANES>(s1);
-                    const float inv = rsqrtf(s1 * inv_dk + a.eps);
-                    float k2 = 0.0f;
-                    if constexpr (BACK) k2 = team_sum<LANES>(s2) * inv_dk * inv * inv;
-#pragma unroll
-                    for (int j = 0; j < PIECES; ++j) {
-                        float o[N];
-                        if constexpr (BACK) {
-#pragma unroll
-                            for (int e = 0; e < N; ++e) {
-                                o[e] = inv * (gv[u][j][e] * w[r][j][e] - xv[u][j][e] * k2);
-                                dw[r][j][e] += gv[u][j][e] * (xv[u][j][e] * inv);
-                            }
-                        } else {
-#pragma unroll
-                            for (int e = 0; e < N; e += 2) {
-                                const float y0 = xv[u][j][e] * inv * w[r][j][e], y1 = xv[u][j][e + 1] * inv * w[r][j][e + 1];
-                                o[e] = y0;
-                                o[e + 1] = y1;
-                                if (turn) rope_rotate(y0, y1, cs[j][e], cs[j][e + 1], o[e], o[e + 1]);
-                            }
-                        }
-                        const int c = (j * LANES + tl) * N;
-                        if (h < H && c < a.dk) Piece<T, N>::store(y + h * a.dk + c, o);
-                    }
-                }
+            for (int i = 0; i < Piece<T, N>::P; ++i) {
+                wc[j].even[i] = f2_mul(w[j].even[i], cs.even[i]);
+                wc[j].odd[i] = f2_mul(w[j].odd[i], cs.even[i]);
+                ws[j].even[i] = f2_mul(w[j].even[i], cs.odd[i]);
+                ws[j].odd[i] = f2_neg(f2_mul(w[j].odd[i], cs.odd[i]));
             }
         }
     }
-    if constexpr (BACK) {
-        if (a.partial == nullptr) return;
-        // teams of a warp, then the warps of the block, in a fixed order
-        __shared__ float red[WARPS][PIECES * LANES * N];
+    const float inv_dk = 1.0f / static_cast<float>(a.dk);
 #pragma unroll
-        for (int r = 0; r < 2; ++r) {
+    for (int u = 0; u < UU; ++u) {
+        const int h = h0 + u * k.step;
+        if (F == ANY && first + u * k.step >= heads) break;  // the same for the whole warp
+        const bool turn = F == FULL_TURN || (F == ANY && h < k.rot);
+        uint64_t sq = 0;
+        Piece<T, N> v[PIECES];
 #pragma unroll
-            for (int j = 0; j < PIECES; ++j)
+        for (int j = 0; j < PIECES; ++j) {
+            v[j] = Piece<T, N>(raw[u][j]);
 #pragma unroll
-                for (int e = 0; e < N; ++e) {
-                    float v = dw[r][j][e];
+            for (int i = 0; i < Piece<T, N>::P; ++i) sq = f2_fma(v[j].odd[i], v[j].odd[i], f2_fma(v[j].even[i], v[j].even[i], sq));
+        }
+        const uint64_t inv = f2_both(rsqrtf(team_sum<LANES>(f2_sum(sq)) * inv_dk + a.eps));
 #pragma unroll
-                    for (int o = 16; o >= LANES; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-                    if (team == 0) red[threadIdx.x >> 5][(j * LANES + tl) * N + e] = v;
+        for (int j = 0; j < PIECES; ++j) {
+            Piece<T, N> o;
+#pragma unroll
+            for (int i = 0; i < Piece<T, N>::P; ++i) {
+                if (turn) {
+                    o.even[i] = f2_mul(inv, f2_fma(v[j].odd[i], ws[j].odd[i], f2_mul(v[j].even[i], wc[j].even[i])));
+                    o.odd[i] = f2_mul(inv, f2_fma(v[j].odd[i], wc[j].odd[i], f2_mul(v[j].even[i], ws[j].even[i])));
+                } else {
+                    o.even[i] = f2_mul(inv, f2_mul(v[j].even[i], w[j].even[i]));
+                    o.odd[i] = f2_mul(inv, f2_mul(v[j].odd[i], w[j].odd[i]));
                 }
-            __syncthreads();
-            for (int c = threadIdx.x; c < a.dk; c += THREADS) {
-                float v = 0.0f;
-#pragma unroll
-                for (int k = 0; k < WARPS; ++k) v += red[k][c];
-                a.partial[(static_cast<int64_t>(blockIdx.x) * 2 + r) * a.dk + c] = v;
             }
-            __syncthreads();
+            if (F != ANY || (token && h < heads && at.col(j) < a.dk)) o.store(y + u * hop + j * (LANES * N));
         }
     }
 }
 
-// dw[r][c] += sum of the blocks' partials, in a fixed order: a block owns 32 columns, its 32 warps
-// take every 32nd partial and are then added in ascending order.
+template <typename T, int N, int LANES, int PIECES>
+__global__ void __launch_bounds__(THREADS, PIECES == 1 ? 4 : 1)
+qk_norm_rope_fwd_kernel(QkArgs a) {
+    constexpr int TEAMS = 32 / LANES;
+    const Place<T, N, LANES, PIECES> at;
+    const bool keys = static_cast<int>(blockIdx.y) >= a.kind[0].rounds;
+    const Kind& k = a.kind[keys];
+    const int first = (static_cast<int>(blockIdx.y) - (keys ? a.kind[0].rounds : 0)) * k.step * k.u;
+    const int64_t group = static_cast<int64_t>(blockIdx.x) * WARPS + (threadIdx.x >> 5);
+    if (group >= k.groups) return;
+    const int per = TEAMS / k.step;
+    const int64_t t = group * per + at.team / k.step;
+    with_shape<T, N, LANES, PIECES>(a, k, first, (group + 1) * per <= a.T, [&](auto shape) { forward_task(a, k, at, t, first, shape); });
+}
+
+// One task of the backward; adds the thread's share of dw.
+template <typename T, int N, int LANES, int PIECES, Form F, int UU>
+__device__ __forceinline__ void backward_task(const QkArgs& a, const Kind& k, const Place<T, N, LANES, PIECES>& at, const T* x,
+                                              const T* g, T* y, int first, bool token, int64_t p, const Piece<T, N> (&w)[PIECES],
+                                              Piece<T, N> (&dw)[PIECES], Shape<F, UU>) {
+    const int h0 = first + at.team % k.step, hop = k.step * a.dk;
+    const int heads = min(k.heads, first + k.step * k.u);  // ANY: where the round ends
+    uint4 xr[UU][PIECES], gr[UU][PIECES];
+#pragma unroll
+    for (int u = 0; u < UU; ++u)
+#pragma unroll
+        for (int j = 0; j < PIECES; ++j) {
+            if (F == ANY) xr[u][j] = gr[u][j] = make_uint4(0, 0, 0, 0);
+            if (F != ANY || (token && h0 + u * k.step < heads && at.col(j) < a.dk)) {
+                xr[u][j] = Piece<T, N>::load_raw(x + u * hop + j * (LANES * N));
+                gr[u][j] = Piece<T, N>::load_raw(g + u * hop + j * (LANES * N));
+            }
+        }
+    Piece<T, N> cs[PIECES];
+    if (F == FULL_TURN || (F == ANY && a.pos)) {
+        const float* row = table_row(a, p);
+#pragma unroll
+        for (int j = 0; j < PIECES; ++j) cs[j].table(row, at.col(j), a.dk);  // cos in even, sin in odd
+    }
+    const float inv_dk = 1.0f / static_cast<float>(a.dk);
+#pragma unroll
+    for (int u = 0; u < UU; ++u) {
+        const int h = h0 + u * k.step;
+        if (F == ANY && first + u * k.step >= heads) break;  // the same for the whole warp
+        const bool turn = F == FULL_TURN || (F == ANY && h < k.rot);
+        Piece<T, N> xv[PIECES], gv[PIECES];
+        uint64_t q1 = 0, q2 = 0;
+#pragma unroll
+        for (int j = 0; j < PIECES; ++j) {
+            xv[j] = Piece<T, N>(xr[u][j]);
+            gv[j] = Piece<T, N>(gr[u][j]);
+#pragma unroll
+            for (int i = 0; i < Piece<T, N>::P; ++i) {
+                if (turn) {  // by the negative angle
+                    const uint64_t e = gv[j].even[i], o = gv[j].odd[i];
+                    gv[j].even[i] = f2_fma(o, cs[j].odd[i], f2_mul(e, cs[j].even[i]));
+                    gv[j].odd[i] = f2_fma(f2_neg(e), cs[j].odd[i], f2_mul(o, cs[j].even[i]));
+                }
+                q1 = f2_fma(xv[j].odd[i], xv[j].odd[i], f2_fma(xv[j].even[i], xv[j].even[i], q1));
+                q2 = f2_fma(f2_mul(gv[j].even[i], w[j].even[i]), xv[j].even[i], q2);
+                q2 = f2_fma(f2_mul(gv[j].odd[i], w[j].odd[i]), xv[j].odd[i], q2);
+            }
+        }
+        const float inv = rsqrtf(team_sum<LANES>(f2_sum(q1)) * inv_dk + a.eps);
+        const uint64_t inv2 = f2_both(inv), k2 = f2_both(-team_sum<LANES>(f2_sum(q2)) * inv_dk * inv * inv);
+#pragma unroll
+        for (int j = 0; j < PIECES; ++j) {
+            Piece<T, N> o;
+#pragma unroll
+            for (int i = 0; i < Piece<T, N>::P; ++i) {
+                o.even[i] = f2_mul(inv2, f2_fma(xv[j].even[i], k2, f2_mul(gv[j].even[i], w[j].even[i])));
+                o.odd[i] = f2_mul(inv2, f2_fma(xv[j].odd[i], k2, f2_mul(gv[j].odd[i], w[j].odd[i])));
+                dw[j].even[i] = f2_fma(f2_mul(gv[j].even[i], xv[j].even[i]), inv2, dw[j].even[i]);
+                dw[j].odd[i] = f2_fma(f2_mul(gv[j].odd[i], xv[j].odd[i]), inv2, dw[j].odd[i]);
+            }
+            if (F != ANY || (token && h < heads && at.col(j) < a.dk)) o.store(y + u * hop + j * (LANES * N));
+        }
+    }
+}
+
+// A warp keeps one round of heads of one kind and walks the groups of tokens, so that what depends on
+// the heads is set up once and a thread's share of dw stays in registers. The next group's position is
+// fetched a group ahead: only one memory latency (data beside table) stands in a group's way.
+template <typename T, int N, int LANES, int PIECES>
+__global__ void __launch_bounds__(THREADS, PIECES == 1 ? 2 : 1)
+qk_norm_rope_bwd_kernel(QkArgs a) {
+    constexpr int TEAMS = 32 / LANES;
+    __shared__ float red[WARPS][PIECES * LANES * N];
+    const Place<T, N, LANES, PIECES> at;
+    const bool keys = static_cast<int>(blockIdx.x) >= a.kind[0].blocks;
+    const Kind& k = a.kind[keys];
+    const int warp = (blockIdx.x - (keys ? a.kind[0].blocks : 0)) * WARPS + (threadIdx.x >> 5);
+    const int walkers = k.blocks * WARPS / k.rounds;  // warps per round; the remainder has no work
+    const int round = warp / walkers, first = round * k.step * k.u;
+    const int per = TEAMS / k.step, sub = at.team / k.step;
+    Piece<T, N> dw[PIECES], w[PIECES];
+#pragma unroll
+    for (int j = 0; j < PIECES; ++j) {
+        w[j].table(k.w, at.col(j), a.dk);
+#pragma unroll
+        for (int i = 0; i < Piece<T, N>::P; ++i) dw[j].even[i] = dw[j].odd[i] = 0;
+    }
+    if (round < k.rounds) {
+        int64_t t = static_cast<int64_t>(warp % walkers) * per + sub;
+        const int64_t end = (k.groups - 1) * per + sub, hop = static_cast<int64_t>(walkers) * per;
+        const int c0 = (first + at.team % k.step) * a.dk + at.tl * N;
+        const T* x = static_cast<const T*>(k.x) + t * k.ldx + c0;
+        const T* g = static_cast<const T*>(k.g) + t * k.ldg + c0;
+        T* y = static_cast<T*>(k.y) + t * k.ldy + c0;
+        const bool turns = a.pos != nullptr;
+        int64_t p = turns && t < a.T ? a.pos[t] : 0;
+        with_shape<T, N, LANES, PIECES>(a, k, first, a.T % per == 0, [&](auto shape) {
+            for (; t <= end; t += hop, x += hop * k.ldx, g += hop * k.ldg, y += hop * k.ldy) {
+                const int64_t ahead = turns && t + hop < a.T ? a.pos[t + hop] : 0;
+                backward_task(a, k, at, x, g, y, first, t < a.T, p, w, dw, shape);
+                p = ahead;
+            }
+        });
+    }
+    if (a.partial == nullptr) return;
+    // teams of a warp, then the warps of the block, in a fixed order
+#pragma unroll
+    for (int j = 0; j < PIECES; ++j)
+#pragma unroll
+        for (int e = 0; e < N; ++e) {
+            float lo, hi;
+            f2_unpack(e % 2 == 0 ? dw[j].even[e / 4] : dw[j].odd[e / 4], lo, hi);
+            float v = e % 4 < 2 ? lo : hi;
+#pragma unroll
+            for (int o = 16; o >= LANES; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+            if (at.team == 0) red[threadIdx.x >> 5][at.col(j) + e] = v;
+        }
+    __syncthreads();
+    for (int c = threadIdx.x; c < a.dk; c += THREADS) {
+        float v = 0.0f;
+#pragma unroll
+        for (int q = 0; q < WARPS; ++q) v += red[q][c];
+        a.partial[static_cast<int64_t>(blockIdx.x) * a.dk + c] = v;
+    }
+}
+
+// dw += sum of the kind's partials, in a fixed order: a block owns 32 columns, its 32 warps take every
+// 32nd partial and are then added in ascending order.
 __global__ void __launch_bounds__(1024)
-qk_gain_grad_kernel(const float* __restrict__ partial, int blocks, int dk, float* __restrict__ dwq, float* __restrict__ dwk) {
+qk_gain_grad_kernel(const float* __restrict__ partial, int nq, int nk, int dk, float* __restrict__ dwq, float* __restrict__ dwk) {
     __shared__ float red[32][33];
-    const int r = blockIdx.y, c = blockIdx.x * 32 + threadIdx.x;
-    float* out = r == 0 ? dwq : dwk;
+    const int c = blockIdx.x * 32 + threadIdx.x, n = blockIdx.y == 0 ? nq : nk;
+    float* out = blockIdx.y == 0 ? dwq : dwk;
     if (out == nullptr) return;
+    if (blockIdx.y == 1) partial += static_cast<int64_t>(nq) * dk;
     float v = 0.0f;
     if (c < dk)
-        for (int b = threadIdx.y; b < blocks; b += 32) v += partial[(static_cast<int64_t>(b) * 2 + r) * dk + c];
+        for (int b = threadIdx.y; b < n; b += 32) v += partial[static_cast<int64_t>(b) * dk + c];
     red[threadIdx.y][threadIdx.x] = v;
     __syncthreads();
     if (threadIdx.y == 0 && c < dk) {
@@ -230,30 +405,49 @@ qk_gain_grad_kernel(const float* __restrict__ partial, int blocks, int dk, float
     }
 }
 
-int bwd_blocks_most() { return sm_count() * 4; }
-
-// Warps that share a token: as many as keep the grid full when there are few tokens, never more than
-// the token has head groups of one warp.
-int parts_for(int64_t T, int Hq, int Hkv, int teams) {
-    const int groups = std::max((Hq + teams * U - 1) / (teams * U), (Hkv + teams * U - 1) / (teams * U));
-    const int64_t want = (static_cast<int64_t>(sm_count()) * 16 + T - 1) / T;
-    return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(groups, want)));
+// Blocks of the backward: one resident wave at 128 registers, shared out by heads, at least a warp
+// for every round of a kind.
+int blocks_of(int heads, int others, int rounds) {
+    if (heads == 0) return 0;
+    const int64_t wave = static_cast<int64_t>(sm_count()) * 2;
+    const int share = static_cast<int>(std::max<int64_t>(1, wave * heads / (static_cast<int64_t>(heads) + others)));
+    return std::max(share, (rounds + WARPS - 1) / WARPS);
+}
+void cut(QkArgs& a, int teams) {
+    for (Kind& k : a.kind) {
+        k.step = 1;
+        while (k.step < teams && k.step < k.heads) k.step *= 2;
+        // a round of U heads per team; fewer where that leaves no round half empty
+        k.u = k.heads % (k.step * U) == 0 || k.heads > k.step * U ? U : (k.heads % (k.step * 2) == 0 ? 2 : (k.heads <= k.step ? 1 : U));
+        k.rounds = (k.heads + k.step * k.u - 1) / (k.step * k.u);
+        k.groups = (a.T + teams / k.step - 1) / (teams / k.step);
+    }
 }
 
 template <typename T, int N, int LANES, int PIECES, bool BACK>
-int launch(cudaStream_t st, QkArgs a, int* blocks_out) {
-    a.parts = parts_for(a.T, a.heads[0], a.heads[1], 32 / LANES);
-    const int64_t need = (a.T * a.parts + WARPS - 1) / WARPS;
-    const int64_t cap = BACK ? bwd_blocks_most() : static_cast<int64_t>(sm_count()) * 16;
-    const int blocks = static_cast<int>(std::min(need, cap));
-    *blocks_out = blocks;
-    qk_norm_rope_kernel<T, N, LANES, PIECES, BACK><<<blocks, THREADS, 0, st>>>(a);
+int launch(cudaStream_t st, QkArgs a, int (&blocks)[2]) {
+    cut(a, 32 / LANES);
+    if constexpr (BACK) {
+        for (int r = 0; r < 2; ++r) {
+            Kind& k = a.kind[r];
+            k.blocks = blocks_of(k.heads, a.kind[1 - r].heads, k.rounds);
+            // a few tokens need no full wave
+            if (k.blocks > 0) k.blocks = static_cast<int>(std::min<int64_t>(k.blocks, (k.groups * k.rounds + WARPS - 1) / WARPS));
+            blocks[r] = k.blocks;
+        }
+        qk_norm_rope_bwd_kernel<T, N, LANES, PIECES><<<static_cast<unsigned>(blocks[0] + blocks[1]), THREADS, 0, st>>>(a);
+    } else {
+        const int64_t gx = (std::max(a.kind[0].heads ? a.kind[0].groups : 0, a.kind[1].heads ? a.kind[1].groups : 0) + WARPS - 1) / WARPS;
+        const int gy = a.kind[0].rounds + a.kind[1].rounds;
+        PK_REQUIRE(gx <= 0x7fffffff && gy <= 65535, "too many rows or heads");
+        qk_norm_rope_fwd_kernel<T, N, LANES, PIECES><<<dim3(static_cast<unsigned>(gx), gy), THREADS, 0, st>>>(a);
+    }
     PK_LAUNCH_CHECK();
     return PK_OK;
 }
 
 template <typename T, bool BACK>
-int dispatch(cudaStream_t st, const QkArgs& a, bool wide, int* blocks) {
+int dispatch(cudaStream_t st, const QkArgs& a, bool wide, int (&blocks)[2]) {
     constexpr int N = Vec<T>::N;
     if (wide) {
         const int lanes = (a.dk + N - 1) / N;
@@ -308,28 +502,26 @@ int pk_qk_norm_rope_fwd(void* stream, int dtype, const void* q, int64_t ldq, con
     PK_REQUIRE(Hkv == 0 || (k && ko && wk), "null pointer");
     const bool turn = rot_q + rot_k > 0;
     PK_REQUIRE(!turn || (pos && cos_sin && n_pos > 0), "the rotation needs positions and a table");
-    PK_REQUIRE(!turn || (reinterpret_cast<uintptr_t>(cos_sin) & 7u) == 0, "the table must be 8-byte aligned");
     PK_REQUIRE((q != qo || ldq == ldqo) && (k != ko || ldk == ldko), "in place needs equal row strides");
     QkArgs a{};
-    a.x[0] = q; a.x[1] = k;
-    a.y[0] = qo; a.y[1] = ko;
-    a.ldx[0] = ldq; a.ldx[1] = ldk;
-    a.ldy[0] = ldqo; a.ldy[1] = ldko;
-    a.w[0] = wq ? wq : wk; a.w[1] = wk ? wk : wq;
-    a.heads[0] = Hq; a.heads[1] = Hkv;
-    a.rot[0] = rot_q; a.rot[1] = rot_k;
-    a.dk = head_dim; a.eps = eps; a.pos = pos; a.cs = cos_sin; a.n_pos = n_pos; a.T = T;
+    a.kind[0] = {q, nullptr, qo, ldq, 0, ldqo, wq, Hq, rot_q, 0, 0, 0, 0, 0};
+    a.kind[1] = {k, nullptr, ko, ldk, 0, ldko, wk, Hkv, rot_k, 0, 0, 0, 0, 0};
+    a.dk = head_dim; a.eps = eps; a.pos = turn ? pos : nullptr; a.cs = cos_sin; a.n_pos = n_pos; a.T = T;
     const int vec = dtype == PK_F32 ? 4 : 8;
-    const bool wide = head_dim % vec == 0 && (Hq == 0 || (rows_aligned(q, ldq, dtype) && rows_aligned(qo, ldqo, dtype))) &&
+    const bool wide = head_dim % vec == 0 && (!turn || aligned16(cos_sin)) && (Hq == 0 || aligned16(wq)) && (Hkv == 0 || aligned16(wk)) &&
+                      (Hq == 0 || (rows_aligned(q, ldq, dtype) && rows_aligned(qo, ldqo, dtype))) &&
                       (Hkv == 0 || (rows_aligned(k, ldk, dtype) && rows_aligned(ko, ldko, dtype)));
-    int blocks = 0;
-    return dtype == PK_F32 ? dispatch<float, false>(as_stream(stream), a, wide, &blocks)
-                           : dispatch<bf16, false>(as_stream(stream), a, wide, &blocks);
+    int blocks[2] = {};
+    return dtype == PK_F32 ? dispatch<float, false>(as_stream(stream), a, wide, blocks)
+                           : dispatch<bf16, false>(as_stream(stream), a, wide, blocks);
 }
 
 size_t pk_qk_norm_rope_bwd_scratch_bytes(int64_t T, int Hq, int Hkv, int head_dim) {
-    (void)T; (void)Hq; (void)Hkv;
-    return static_cast<size_t>(bwd_blocks_most()) * 2 * static_cast<size_t>(std::max(head_dim, 0)) * sizeof(float);
+    (void)T;
+    if (Hq < 0 || Hkv < 0 || head_dim <= 0) return 0;
+    // the most blocks of any form: a head per round makes the most rounds
+    const size_t blocks = static_cast<size_t>(blocks_of(Hq, Hkv, Hq)) + static_cast<size_t>(blocks_of(Hkv, Hq, Hkv));
+    return blocks * static_cast<size_t>(head_dim) * sizeof(float);
 }
 
 int pk_qk_norm_rope_bwd(void* stream, int dtype, const void* dqo, int64_t lddqo, const void* dko, int64_t lddko,
@@ -347,33 +539,25 @@ int pk_qk_norm_rope_bwd(void* stream, int dtype, const void* dqo, int64_t lddqo,
     PK_REQUIRE(Hkv == 0 || (k && dko && dk && wk), "null pointer");
     const bool turn = rot_q + rot_k > 0;
     PK_REQUIRE(!turn || (pos && cos_sin && n_pos > 0), "the rotation needs positions and a table");
-    PK_REQUIRE(!turn || (reinterpret_cast<uintptr_t>(cos_sin) & 7u) == 0, "the table must be 8-byte aligned");
     PK_REQUIRE((dqo != dq || lddqo == lddq) && (dko != dk || lddko == lddk), "in place needs equal row strides");
     const bool gains = dwq != nullptr || dwk != nullptr;
     PK_REQUIRE(!gains || scratch, "the gains' gradients need scratch");
     PK_REQUIRE(!gains || dwq != dwk, "the two gains' gradients must be two buffers");
     QkArgs a{};
-    a.x[0] = q; a.x[1] = k;
-    a.g[0] = dqo; a.g[1] = dko;
-    a.y[0] = dq; a.y[1] = dk;
-    a.ldx[0] = ldq; a.ldx[1] = ldk;
-    a.ldg[0] = lddqo; a.ldg[1] = lddko;
-    a.ldy[0] = lddq; a.ldy[1] = lddk;
-    a.w[0] = wq ? wq : wk; a.w[1] = wk ? wk : wq;
-    a.heads[0] = Hq; a.heads[1] = Hkv;
-    a.rot[0] = rot_q; a.rot[1] = rot_k;
-    a.dk = head_dim; a.eps = eps; a.pos = pos; a.cs = cos_sin; a.n_pos = n_pos; a.T = T;
+    a.kind[0] = {q, dqo, dq, ldq, lddqo, lddq, wq, Hq, rot_q, 0, 0, 0, 0, 0};
+    a.kind[1] = {k, dko, dk, ldk, lddko, lddk, wk, Hkv, rot_k, 0, 0, 0, 0, 0};
+    a.dk = head_dim; a.eps = eps; a.pos = turn ? pos : nullptr; a.cs = cos_sin; a.n_pos = n_pos; a.T = T;
     a.partial = gains ? static_cast<float*>(scratch) : nullptr;
     const int vec = dtype == PK_F32 ? 4 : 8;
-    const bool wide = head_dim % vec == 0 &&
+    const bool wide = head_dim % vec == 0 && (!turn || aligned16(cos_sin)) && (Hq == 0 || aligned16(wq)) && (Hkv == 0 || aligned16(wk)) &&
                       (Hq == 0 || (rows_aligned(q, ldq, dtype) && rows_aligned(dqo, lddqo, dtype) && rows_aligned(dq, lddq, dtype))) &&
                       (Hkv == 0 || (rows_aligned(k, ldk, dtype) && rows_aligned(dko, lddko, dtype) && rows_aligned(dk, lddk, dtype)));
-    int blocks = 0;
-    const int rc = dtype == PK_F32 ? dispatch<float, true>(as_stream(stream), a, wide, &blocks)
-                                   : dispatch<bf16, true>(as_stream(stream), a, wide, &blocks);
+    int blocks[2] = {};
+    const int rc = dtype == PK_F32 ? dispatch<float, true>(as_stream(stream), a, wide, blocks)
+                                   : dispatch<bf16, true>(as_stream(stream), a, wide, blocks);
     if (rc != PK_OK || !gains) return rc;
     qk_gain_grad_kernel<<<dim3((head_dim + 31) / 32, 2), dim3(32, 32), 0, as_stream(stream)>>>(
-        static_cast<const float*>(scratch), blocks, head_dim, dwq, dwk);
+        static_cast<const float*>(scratch), blocks[0], blocks[1], head_dim, dwq, dwk);
     PK_LAUNCH_CHECK();
     return PK_OK;
 }

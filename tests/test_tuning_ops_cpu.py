@@ -87,7 +87,6 @@ def test_qk_norm_rope_refusals(pk):
     refused(pk, call(wq=None), b"null")
     refused(pk, call(pos=None), b"table")
     refused(pk, call(n_pos=0), b"table")
-    refused(pk, call(cs=ctypes.c_void_p(4)), b"aligned")
     refused(pk, call(qo=P, ldqo=80), b"in place")
     assert call(T=0) == 0
     b = pk.pk_qk_norm_rope_bwd
