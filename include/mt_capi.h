@@ -33,6 +33,7 @@ int mt_sync(void);
 /* spec: "key=value;key=value;..." with keys
  *   family   llama | gpt2 | flex
  *   vocab d layers heads kv_heads dff nctx theta tie rope_all qlora rank alpha seed
+ *   qk_norm (0|1: RMS norm of every query and key head before the rotation)   [llama, block]
  *   norm (layernorm|rmsnorm)  act (gelu|relu|swiglu)  pos (learned|sinusoidal)   [flex]
  *   ckpt (0|1: per-block activation checkpointing)
  *   pack (0|1, default 1: parameters, gradients and bf16 shadows in flat buffers)
@@ -59,6 +60,29 @@ int mt_model_grad_get(void* model, int64_t index, float* out_h, int* has_grad_h)
  * UNSCALED mean loss (read back after the backward was enqueued). */
 int mt_model_step(void* model, const int32_t* ids_h, const int32_t* targets_h, int64_t n, int64_t seq_len,
                   float loss_scale, int do_backward, float* loss_h);
+/* ---- preference / policy tuning (no counterpart in the reference, which trains on cross entropy) ----
+ * All three take the token ids and per-row targets of mt_model_step; weight_h (may be null: all ones) marks
+ * the rows that count -- rows of weight 0 (prompt, padding) are left out, whatever their target (-100 is
+ * usual). The head runs fused over row chunks like the cross entropy.
+ * mt_model_token_logprob: logp_h[n] = log-probability of every row's target (0 where the weight is 0), no
+ * gradient: the reference policy's values, or the old policy's before an update.
+ * mt_model_policy_step: loss = sum of weight * (-min(r A, clamp(r, 1 - clip_lo, 1 + clip_hi) A) + kl_coef (e^u - u - 1)),
+ * r = exp(logp - old_logp), u = ref_logp - logp; old_logp_h null: r = 1; ref_logp_h null: no KL term. The weights
+ * normalise the sum. logp_h, kl_h [n] (may be null) receive the rows' values.
+ * mt_model_preference_step: loss = mean over the n_pairs pairs of the paired log-ratio loss; seq_h holds
+ * 2 n_pairs + 1 ascending row offsets (sequences 2 i and 2 i + 1: chosen and rejected answer of pair i; rows
+ * outside do not count). pair_loss_h, margin_h [n_pairs] may be null.
+ * loss_scale, do_backward and *loss_h as in mt_model_step. */
+int mt_model_token_logprob(void* model, const int32_t* ids_h, const int32_t* targets_h, const float* weight_h, int64_t n,
+                           int64_t seq_len, float* logp_h);
+int mt_model_policy_step(void* model, const int32_t* ids_h, const int32_t* targets_h, int64_t n, int64_t seq_len,
+                         const float* old_logp_h, const float* ref_logp_h, const float* advantage_h, const float* weight_h,
+                         float clip_lo, float clip_hi, float kl_coef, float loss_scale, int do_backward, float* loss_h,
+                         float* logp_h, float* kl_h);
+int mt_model_preference_step(void* model, const int32_t* ids_h, const int32_t* targets_h, int64_t n, int64_t seq_len,
+                             const float* ref_logp_h, const float* weight_h, const int32_t* seq_h, int64_t n_pairs, float beta,
+                             float label_smoothing, float loss_scale, int do_backward, float* loss_h, float* pair_loss_h,
+                             float* margin_h);
 /* Variables alive between forward and backward of the last mt_model_step (the
  * reference's memory receipt for checkpointing, include/microtorch/autograd.hpp:61-64). */
 /* ---- one Llama block on its own (spec family=block; keys d, heads, kv_heads, dff, theta,
@@ -80,6 +104,13 @@ int mt_model_live_after_forward(void* model, int64_t* n_h);
 /* AdamW with the reference's defaults unless set (lr 1e-3, betas 0.9/0.999, eps 1e-8, wd 0.01). */
 int mt_model_set_adamw(void* model, float lr, float beta1, float beta2, float eps, float weight_decay);
 int mt_model_optimizer_step(void* model);
+/* Bits of the stored moments, 32 (default) or 8 (2.06 bytes per parameter instead of 8, see pk_adamw_multi);
+ * before the first step. mt_model_save / load and the state entries below keep working: the moments are
+ * converted to fp32 and back without loss, and a restored run continues bit-identically. */
+int mt_model_set_adamw_state_bits(void* model, int bits);
+/* Learning-rate factor and weight decay of one parameter (index of mt_model_param_info) from the next step on;
+ * the others keep (1, the decay of mt_model_set_adamw). */
+int mt_model_set_param_rates(void* model, int64_t index, float lr_mult, float weight_decay);
 
 /* Checkpoint files in the safetensors layout of the reference (src/safetensors.cpp:12-94: 8-byte
  * little-endian header length, JSON header, raw fp32 tensors in sorted name order, header padded

@@ -10,6 +10,8 @@
 //                   [T,3d] layout); true = every head is rotated
 //   qlora           frozen Q8_0 base weights (embedding and norm gains frozen too)
 //                   with trainable LoRA adapters on q_proj and v_proj
+//   qk_norm         RMS norm of every query and key head before the rotation, gains
+//                   "self_attn.q_norm.weight" / "k_norm.weight" [1, head_dim] shared by the heads
 // The block is written against the fused ops: one attention node for all heads,
 // in-place rotary on the projection outputs, residual adds in the GEMM epilogues.
 #include "microtorch/nn.hpp"
@@ -28,6 +30,7 @@ struct LlamaConfig {
     size_t n_kv_heads = 0;
     bool rope_all_heads = false;
     bool qlora = false;
+    bool qk_norm = false;
     size_t lora_rank = 16;
     float lora_alpha = 32.0f;
 };
@@ -53,6 +56,7 @@ public:
     Var forward(const Var& x, const std::vector<int>& positions, size_t seq_len = 0) const;
 
     Var ln1_w, ln2_w;
+    Var q_norm_w, k_norm_w;  // null unless qk_norm
     std::shared_ptr<Projection> q_proj, k_proj, v_proj, o_proj;
     std::shared_ptr<Projection> gate_proj, up_proj, down_proj;
     size_t H, Hkv, dk;
@@ -69,6 +73,9 @@ public:
     // cross_entropy(forward(ids), targets) with the head and the loss fused over row chunks.
     Var loss(const std::vector<int>& ids, const std::vector<int>& targets, size_t seq_len = 0,
              size_t chunk_rows = 16384) const;
+
+    // Weight of the vocabulary projection and whether it is stored [vocab, d] (the tied embedding).
+    std::pair<Var, bool> head() const;
 
     // QLoRA mode: takes the frozen base (projections, embedding, norm gains) from the tensors of
     // a DENSE model of the same shape, named as that model registers them ("layers.0.self_attn.

@@ -172,6 +172,13 @@ public:
     // Before the first step the moments read as zero, and imported moments are held on the
     // host until the step that creates the device state.
     void set_steps_taken(long t) { t_ = t; }
+    // 32 (default) or 8: bits of the stored moments (pk_adamw_multi: E4M3 codes with a power-of-two scale
+    // per 32 elements, 2.06 bytes per parameter instead of 8). Before the first step.
+    void set_state_bits(int bits);
+    int state_bits() const { return bits_; }
+    // Learning-rate factor and weight decay of one parameter (the reference steps and decays all alike,
+    // which is (1, weight_decay)); e.g. no decay for norm gains. Takes effect with the next step.
+    void set_rates(size_t index, float lr_mult, float weight_decay);
     void export_state(size_t index, float* m_h, float* v_h);
     void import_state(size_t index, const float* m_h, const float* v_h);
 
@@ -182,17 +189,25 @@ private:
         float* g = nullptr;
         void* shadow = nullptr;
         size_t n = 0;
-        Tensor m, v;
+        Tensor m, v;      // fp32 moments, or the codes of 8-bit ones
+        Tensor ms, vs;    // scales of 8-bit moments
     };
     void build_runs();
+    // The many-tensor plan of what is stepped now; made again when that changes.
+    void* plan();
+    void put_state(const Run& run, size_t offset, size_t n, const float* m_h, const float* v_h);
     bool locate(size_t index, size_t* run, size_t* offset) const;
     struct Pending { std::vector<float> m, v; };
     std::map<size_t, Pending> pending_;
     std::vector<Var> params_;
     std::vector<Run> runs_;
-    bool runs_built_ = false;
     float b1_, b2_, eps_, wd_;
     long t_ = 0;
+    int bits_ = 32;
+    struct Rates { float lr_mult, weight_decay; };
+    std::map<size_t, Rates> rates_;        // parameters with rates of their own
+    std::shared_ptr<void> plan_;
+    std::vector<std::vector<uint64_t>> planned_;  // what the plan was made from
 };
 
 // Inverted dropout layer (reference: include/microtorch/nn.hpp:281-289, src/nn.cpp:479-482):

@@ -35,6 +35,27 @@ Var cross_entropy(const Var& logits, const std::vector<int>& targets);
 // [rows, vocab] logits never exist as a whole; W is [in, out], or [out, in] when transposed_w.
 Var linear_cross_entropy(const Var& h, const Var& W, bool transposed_w, const std::vector<int>& targets,
                          size_t chunk_rows = 16384);
+// ---- preference / policy tuning (no counterpart in the reference) -------------------------------
+// The losses of pk_policy_loss and pk_preference_loss over the rows of h W (or h W^T), chunked like
+// linear_cross_entropy. Empty vectors leave a term out; rows of weight 0 do not count, whatever their
+// target. The policy loss is the SUM of the weighted row losses (the caller's weights normalise it); the
+// preference loss is the mean over the pairs. *logp, *kl, *pair_loss, *margin (may be null) receive host copies.
+struct PolicyTerms {
+    std::vector<float> old_logp, ref_logp, advantage, weight;
+    float clip_lo = 0.2f, clip_hi = 0.2f, kl_coef = 0.0f;
+};
+Var linear_policy_loss(const Var& h, const Var& W, bool transposed_w, const std::vector<int>& targets, const PolicyTerms& terms,
+                       size_t chunk_rows = 16384, std::vector<float>* logp = nullptr, std::vector<float>* kl = nullptr);
+struct PreferenceTerms {
+    std::vector<float> ref_logp, weight;
+    std::vector<int> seq;  // 2 n + 1 ascending row offsets: chosen and rejected answer of every pair in turn
+    float beta = 0.1f, label_smoothing = 0.0f;
+};
+Var linear_preference_loss(const Var& h, const Var& W, bool transposed_w, const std::vector<int>& targets, const PreferenceTerms& terms,
+                           size_t chunk_rows = 16384, std::vector<float>* pair_loss = nullptr, std::vector<float>* margin = nullptr);
+// Log-probability of every row's target under h W, on the host; no gradient.
+std::vector<float> linear_token_logprob(const Var& h, const Var& W, bool transposed_w, const std::vector<int>& targets,
+                                        const std::vector<float>& weight = {}, size_t chunk_rows = 16384);
 // qk is the fused [T, 3d] q|k|v layout. Like the reference (src/ops.cpp:495-511) this
 // rotates the first head_dim columns of q and of k only.
 Var apply_rope(const Var& qk, const std::vector<int>& pos, float theta_base, size_t head_dim);
@@ -69,6 +90,11 @@ Var attention(const Var& q, const Var& k, const Var& v, size_t n_heads, size_t n
 // attention(slice_cols(qkv, 0, d), slice_cols(qkv, d, 2 d), slice_cols(qkv, 2 d, 3 d), n_heads, n_heads, ...)
 // for a packed [T, 3 d] projection, without the slices: the same values, read and written in place.
 Var attention_packed(const Var& qkv, size_t n_heads, size_t seq_len, bool causal);
+// attention(norm_rope(q), norm_rope(k), v, ...) as one node: every head of q and k is RMS-normed with its kind's
+// gain ([1, head_dim], shared by the heads) and the first rot_q / rot_k heads are rotated, in one pass.
+Var attention_qk_norm(const Var& q, const Var& k, const Var& v, const Var& wq, const Var& wk, const std::vector<int>& pos,
+                      float theta_base, size_t rot_q, size_t rot_k, size_t n_heads, size_t n_kv_heads, size_t seq_len, bool causal,
+                      float eps = 1e-5f);
 // Rotates the first `n_rot` heads (width head_dim) of x [T, H*head_dim] IN PLACE and
 // returns a node that shares x's buffer. x must have no other consumer and must be the
 // output of an op whose backward does not read its own output (a linear / matmul).

@@ -3,6 +3,7 @@
 
 #include <cstring>
 #include <fstream>
+#include <functional>
 #include <map>
 #include <sstream>
 #include <stdexcept>
@@ -42,6 +43,7 @@ struct Model {
     std::unique_ptr<nn::AdamW> opt;
     std::unique_ptr<dp::GradientExchange> exchange;   // data-parallel gradient exchange (mt_dp_*)
     float lr = 1e-3f, b1 = 0.9f, b2 = 0.999f, eps = 1e-8f, wd = 0.01f;
+    int state_bits = 32;
     int64_t live_after_fwd = 0;
     size_t loss_chunk = 16384;
     bool accumulate = false;   // mt_model_step keeps the gradients it finds
@@ -58,6 +60,18 @@ struct Model {
         if (llama) return llama->loss(ids, targets, seq_len, loss_chunk);
         if (gpt2) return gpt2->loss(ids, targets, seq_len, loss_chunk);
         return flex->loss(ids, targets, seq_len, loss_chunk);
+    }
+    Var hidden(const std::vector<int>& ids, size_t seq_len) const {
+        if (block) throw std::runtime_error("a block has no token interface: use mt_block_set_input / forward / backward");
+        if (llama) return llama->hidden(ids, seq_len);
+        if (gpt2) return gpt2->hidden(ids, seq_len);
+        return flex->hidden(ids, seq_len);
+    }
+    // Weight of the vocabulary projection, and whether it is stored [vocab, d].
+    std::pair<Var, bool> head() const {
+        if (llama) return llama->head();
+        if (gpt2) return {gpt2->wte->weight, true};
+        return {flex->head->W, false};
     }
     void set_ckpt(bool on) {
         if (llama) llama->checkpoint_blocks = on;
@@ -190,6 +204,7 @@ int mt_model_create(const char* spec, void** out) {
             c.tie_embeddings = r.num("tie", 1) != 0;
             c.rope_all_heads = r.num("rope_all", 0) != 0;
             c.qlora = r.num("qlora", 0) != 0;
+            c.qk_norm = r.num("qk_norm", 0) != 0;
             c.lora_rank = r.num("rank", 16);
             c.lora_alpha = static_cast<float>(r.real("alpha", 32.0));
             r.finish();
@@ -230,6 +245,7 @@ int mt_model_create(const char* spec, void** out) {
             c.d_ff = r.num("dff", 512);
             c.rope_theta = static_cast<float>(r.real("theta", 10000.0));
             c.rope_all_heads = r.num("rope_all", 1) != 0;
+            c.qk_norm = r.num("qk_norm", 0) != 0;
             r.finish();
             m->block = std::make_shared<nn::LlamaBlock>(c, seed);
             m->named = m->block->named_parameters();
@@ -447,6 +463,7 @@ int mt_model_export_gguf(void* h, const char* gguf_path, const char* name, int64
         if (!gguf_path) throw std::runtime_error("null path");
         if (!m->llama) throw std::runtime_error("export_gguf: only the llama family maps onto the GGUF llama layout");
         const nn::LlamaConfig& lc = m->llama->cfg;
+        if (lc.qk_norm) throw std::runtime_error("export_gguf: the layout has no place for query and key norms");
         gguf::LlamaExportConfig c;
         if (name) c.name = name;
         c.context_length = static_cast<uint32_t>(context_length);
@@ -463,36 +480,131 @@ int mt_model_export_gguf(void* h, const char* gguf_path, const char* name, int64
     });
 }
 
+namespace {
+// zero_grad (unless accumulating), forward to a scalar loss, and its reverse pass; the loss's value.
+float run_step(Model* m, const char* what, float loss_scale, bool do_backward, const std::function<Var()>& make_loss) {
+    device::step_begin();
+    float loss_value = 0.0f;
+    if (do_backward) {
+        if (!m->accumulate) zero_grad(m->params);
+        const size_t live0 = live_variables();
+        Var loss = make_loss();
+        m->live_after_fwd = static_cast<int64_t>(live_variables() - live0);
+        Var root = loss_scale == 1.0f ? loss : ops::scale(loss, loss_scale);
+        backward(root);
+        loss_value = loss->data.host()(0, 0);
+    } else {
+        NoGrad ng;
+        Var loss = make_loss();
+        loss_value = loss->data.host()(0, 0);
+    }
+    device::step_end();
+    // The loss readback has synchronised the stream: a kernel whose bounded wait gave up has
+    // left the step's results incomplete, which must not pass for a finished step.
+    int status = 0;
+    device::check(pk_kernel_status(&status, 1), "pk_kernel_status");
+    if (status != 0)
+        throw std::runtime_error(std::string(what) + ": a tensor-core kernel abandoned a bounded wait (status " +
+                                 std::to_string(status) + ", PK_ERR_TIMEOUT = 4); the results of this step are incomplete");
+    return loss_value;
+}
+std::vector<int> ints(const int32_t* p, int64_t n) {
+    if (n < 0 || (n > 0 && !p)) throw std::runtime_error("bad argument");
+    return std::vector<int>(p, p + n);
+}
+std::vector<float> floats(const float* p, int64_t n) { return p ? std::vector<float>(p, p + n) : std::vector<float>(); }
+void give(const std::vector<float>& v, float* out) {
+    if (out && !v.empty()) std::memcpy(out, v.data(), v.size() * sizeof(float));
+}
+// Rows per chunk of the fused heads; a model set to unfused losses takes one chunk.
+size_t chunk_of(const Model* m, int64_t rows) {
+    return m->loss_chunk ? m->loss_chunk : static_cast<size_t>(rows > 0 ? rows : 1);
+}
+}  // namespace
+
 int mt_model_step(void* h, const int32_t* ids_h, const int32_t* targets_h, int64_t n, int64_t seq_len,
                   float loss_scale, int do_backward, float* loss_h) {
     return guard([&] {
         Model* m = M(h);
         if (n < 0 || seq_len < 0) throw std::runtime_error("negative size");
         std::vector<int> ids(ids_h, ids_h + n), targets(targets_h, targets_h + n);
+        const float loss = run_step(m, "mt_model_step", loss_scale, do_backward != 0,
+                                    [&] { return m->loss(ids, targets, static_cast<size_t>(seq_len)); });
+        if (loss_h) *loss_h = loss;
+    });
+}
+
+int mt_model_token_logprob(void* h, const int32_t* ids_h, const int32_t* targets_h, const float* weight_h, int64_t n,
+                           int64_t seq_len, float* logp_h) {
+    return guard([&] {
+        Model* m = M(h);
+        if (seq_len < 0 || n <= 0 || !logp_h) throw std::runtime_error("bad argument");
+        const std::vector<int> ids = ints(ids_h, n), targets = ints(targets_h, n);
         device::step_begin();
-        float loss_value = 0.0f;
-        if (do_backward) {
-            if (!m->accumulate) zero_grad(m->params);
-            const size_t live0 = live_variables();
-            Var loss = m->loss(ids, targets, static_cast<size_t>(seq_len));
-            m->live_after_fwd = static_cast<int64_t>(live_variables() - live0);
-            Var root = loss_scale == 1.0f ? loss : ops::scale(loss, loss_scale);
-            backward(root);
-            loss_value = loss->data.host()(0, 0);
-        } else {
-            NoGrad ng;
-            Var loss = m->loss(ids, targets, static_cast<size_t>(seq_len));
-            loss_value = loss->data.host()(0, 0);
-        }
+        NoGrad ng;
+        Var x = m->hidden(ids, static_cast<size_t>(seq_len));
+        const auto head = m->head();
+        give(ops::linear_token_logprob(x, head.first, head.second, targets, floats(weight_h, n), chunk_of(m, n)), logp_h);
         device::step_end();
-        if (loss_h) *loss_h = loss_value;
-        // The loss readback has synchronised the stream: a kernel whose bounded wait gave up has
-        // left the step's results incomplete, which must not pass for a finished step.
         int status = 0;
         device::check(pk_kernel_status(&status, 1), "pk_kernel_status");
-        if (status != 0)
-            throw std::runtime_error("mt_model_step: a tensor-core kernel abandoned a bounded wait (status " +
-                                     std::to_string(status) + ", PK_ERR_TIMEOUT = 4); the results of this step are incomplete");
+        if (status != 0) throw std::runtime_error("mt_model_token_logprob: a tensor-core kernel abandoned a bounded wait");
+    });
+}
+
+int mt_model_policy_step(void* h, const int32_t* ids_h, const int32_t* targets_h, int64_t n, int64_t seq_len,
+                         const float* old_logp_h, const float* ref_logp_h, const float* advantage_h, const float* weight_h,
+                         float clip_lo, float clip_hi, float kl_coef, float loss_scale, int do_backward, float* loss_h,
+                         float* logp_h, float* kl_h) {
+    return guard([&] {
+        Model* m = M(h);
+        if (seq_len < 0 || n <= 0 || !advantage_h) throw std::runtime_error("bad argument");
+        const std::vector<int> ids = ints(ids_h, n), targets = ints(targets_h, n);
+        ops::PolicyTerms terms;
+        terms.old_logp = floats(old_logp_h, n);
+        terms.ref_logp = floats(ref_logp_h, n);
+        terms.advantage = floats(advantage_h, n);
+        terms.weight = floats(weight_h, n);
+        terms.clip_lo = clip_lo;
+        terms.clip_hi = clip_hi;
+        terms.kl_coef = kl_coef;
+        std::vector<float> logp, kl;
+        const float loss = run_step(m, "mt_model_policy_step", loss_scale, do_backward != 0, [&] {
+            Var x = m->hidden(ids, static_cast<size_t>(seq_len));
+            const auto head = m->head();
+            return ops::linear_policy_loss(x, head.first, head.second, targets, terms, chunk_of(m, n), logp_h ? &logp : nullptr,
+                                           kl_h ? &kl : nullptr);
+        });
+        if (loss_h) *loss_h = loss;
+        give(logp, logp_h);
+        give(kl, kl_h);
+    });
+}
+
+int mt_model_preference_step(void* h, const int32_t* ids_h, const int32_t* targets_h, int64_t n, int64_t seq_len,
+                             const float* ref_logp_h, const float* weight_h, const int32_t* seq_h, int64_t n_pairs, float beta,
+                             float label_smoothing, float loss_scale, int do_backward, float* loss_h, float* pair_loss_h,
+                             float* margin_h) {
+    return guard([&] {
+        Model* m = M(h);
+        if (seq_len < 0 || n <= 0 || n_pairs <= 0) throw std::runtime_error("bad argument");
+        const std::vector<int> ids = ints(ids_h, n), targets = ints(targets_h, n);
+        ops::PreferenceTerms terms;
+        terms.ref_logp = floats(ref_logp_h, n);
+        terms.weight = floats(weight_h, n);
+        terms.seq = ints(seq_h, 2 * n_pairs + 1);
+        terms.beta = beta;
+        terms.label_smoothing = label_smoothing;
+        std::vector<float> pair, margin;
+        const float loss = run_step(m, "mt_model_preference_step", loss_scale, do_backward != 0, [&] {
+            Var x = m->hidden(ids, static_cast<size_t>(seq_len));
+            const auto head = m->head();
+            return ops::linear_preference_loss(x, head.first, head.second, targets, terms, chunk_of(m, n),
+                                               pair_loss_h ? &pair : nullptr, margin_h ? &margin : nullptr);
+        });
+        if (loss_h) *loss_h = loss;
+        give(pair, pair_loss_h);
+        give(margin, margin_h);
     });
 }
 
@@ -570,7 +682,10 @@ int mt_model_set_adamw(void* h, float lr, float b1, float b2, float eps, float w
     });
 }
 static nn::AdamW& optimizer(Model* m) {
-    if (!m->opt) m->opt = std::make_unique<nn::AdamW>(m->params, m->lr, m->b1, m->b2, m->eps, m->wd);
+    if (!m->opt) {
+        m->opt = std::make_unique<nn::AdamW>(m->params, m->lr, m->b1, m->b2, m->eps, m->wd);
+        m->opt->set_state_bits(m->state_bits);
+    }
     return *m->opt;
 }
 // The optimizer is built over the packed order; the state entries use the registration
@@ -581,6 +696,20 @@ static size_t optimizer_index(Model* m, int64_t i) {
     for (size_t k = 0; k < m->params.size(); ++k)
         if (m->params[k] == p) return k;
     throw std::runtime_error("parameter is not trainable");
+}
+int mt_model_set_adamw_state_bits(void* h, int bits) {
+    return guard([&] {
+        Model* m = M(h);
+        if (bits != 8 && bits != 32) throw std::runtime_error("AdamW: state bits must be 8 or 32");
+        if (m->opt) m->opt->set_state_bits(bits);
+        m->state_bits = bits;
+    });
+}
+int mt_model_set_param_rates(void* h, int64_t i, float lr_mult, float weight_decay) {
+    return guard([&] {
+        Model* m = M(h);
+        optimizer(m).set_rates(optimizer_index(m, i), lr_mult, weight_decay);
+    });
 }
 int mt_model_optimizer_step(void* h) {
     return guard([&] { optimizer(M(h)).step(); });

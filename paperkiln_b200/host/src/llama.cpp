@@ -53,6 +53,10 @@ LlamaBlock::LlamaBlock(const LlamaConfig& cfg, unsigned seed)
         ln1_w = reg("input_layernorm.weight", Matrix(1, cfg.d, 1.0f));
         ln2_w = reg("post_attention_layernorm.weight", Matrix(1, cfg.d, 1.0f));
     }
+    if (cfg.qk_norm) {
+        q_norm_w = q ? make_var(Matrix(1, dk, 1.0f), false) : reg("self_attn.q_norm.weight", Matrix(1, dk, 1.0f));
+        k_norm_w = q ? make_var(Matrix(1, dk, 1.0f), false) : reg("self_attn.k_norm.weight", Matrix(1, dk, 1.0f));
+    }
     const size_t r = cfg.lora_rank;
     const float a = cfg.lora_alpha;
     q_proj = mod<Projection>("self_attn.q_proj", cfg.d, H * dk, seed + 1, q, q, r, a);
@@ -67,11 +71,18 @@ LlamaBlock::LlamaBlock(const LlamaConfig& cfg, unsigned seed)
 Var LlamaBlock::forward(const Var& x, const std::vector<int>& pos, size_t seq_len) const {
     // ---- attention sublayer (pre-RMSNorm)
     Var h = ops::rmsnorm(x, ln1_w);
-    // q and k are rotated on their way out of the projection's GEMM
-    Var q = q_proj->forward_rope(h, pos, rope_theta_, dk, rope_all_ ? H : 1);
-    Var k = k_proj->forward_rope(h, pos, rope_theta_, dk, rope_all_ ? Hkv : 1);
-    Var v = v_proj->forward(h);
-    Var a = ops::attention(q, k, v, H, Hkv, seq_len, /*causal=*/true);
+    const size_t rot_q = rope_all_ ? H : 1, rot_k = rope_all_ ? Hkv : 1;
+    Var a;
+    if (q_norm_w) {  // the norm stands between projection and rotation
+        Var q = q_proj->forward(h), k = k_proj->forward(h), v = v_proj->forward(h);
+        a = ops::attention_qk_norm(q, k, v, q_norm_w, k_norm_w, pos, rope_theta_, rot_q, rot_k, H, Hkv, seq_len, /*causal=*/true);
+    } else {
+        // q and k are rotated on their way out of the projection's GEMM
+        Var q = q_proj->forward_rope(h, pos, rope_theta_, dk, rot_q);
+        Var k = k_proj->forward_rope(h, pos, rope_theta_, dk, rot_k);
+        Var v = v_proj->forward(h);
+        a = ops::attention(q, k, v, H, Hkv, seq_len, /*causal=*/true);
+    }
     Var x1 = o_proj->forward_residual(a, x);  // x + attn
     // ---- SwiGLU FFN sublayer
     Var h2 = ops::rmsnorm(x1, ln2_w);
@@ -129,6 +140,15 @@ void Llama::load_frozen_base(const std::map<std::string, Matrix>& dense) {
                 b.ln1_w = make_var(g1, false);
                 b.ln2_w = make_var(g2, false);
             }
+            if (cfg.qk_norm) {
+                const size_t dk = cfg.d / cfg.n_heads;
+                const Matrix& gq = fetch(pre + "self_attn.q_norm.weight", 1, dk);
+                const Matrix& gk = fetch(pre + "self_attn.k_norm.weight", 1, dk);
+                if (pass) {
+                    b.q_norm_w = make_var(gq, false);
+                    b.k_norm_w = make_var(gk, false);
+                }
+            }
             for (const Proj& pr : projs) {
                 Projection& p = *(b.*(pr.member));
                 const Matrix& w = fetch(pre + pr.name + ".weight", p.Wq->rows, p.Wq->cols);
@@ -151,6 +171,10 @@ std::map<std::string, Matrix> Llama::merged_state() const {
         const LlamaBlock& b = *blocks[i];
         out[pre + "input_layernorm.weight"] = b.ln1_w->data.host();
         out[pre + "post_attention_layernorm.weight"] = b.ln2_w->data.host();
+        if (cfg.qk_norm) {
+            out[pre + "self_attn.q_norm.weight"] = b.q_norm_w->data.host();
+            out[pre + "self_attn.k_norm.weight"] = b.k_norm_w->data.host();
+        }
         const std::pair<const char*, const Projection*> projs[] = {
             {"self_attn.q_proj", b.q_proj.get()}, {"self_attn.k_proj", b.k_proj.get()},
             {"self_attn.v_proj", b.v_proj.get()}, {"self_attn.o_proj", b.o_proj.get()},
@@ -194,6 +218,11 @@ Var Llama::forward(const std::vector<int>& ids, size_t seq_len) const {
     // from this GEMM (src/llama.cpp:85-88). No transposed copy of E is made.
     const Var& table = cfg.qlora ? embed_frozen : embed_tokens->weight;
     return ops::linear(h, table, nullptr, nullptr, /*transposed_w=*/true);
+}
+
+std::pair<Var, bool> Llama::head() const {
+    if (lm_head) return {lm_head->W, false};
+    return {cfg.qlora ? embed_frozen : embed_tokens->weight, true};
 }
 
 Var Llama::loss(const std::vector<int>& ids, const std::vector<int>& targets, size_t seq_len, size_t chunk_rows) const {

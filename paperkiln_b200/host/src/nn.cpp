@@ -3,6 +3,7 @@
 // SGD 261-291, AdamW 293-325).
 #include "microtorch/nn.hpp"
 
+#include <cstring>
 #include <random>
 #include <stdexcept>
 
@@ -262,7 +263,8 @@ void AdamW::build_runs() {
         r.shadow = params_[i]->shadow.defined() && params_[i]->shadow.dtype() == DType::BF16 ? params_[i]->shadow.ptr() : nullptr;
         r.n = params_[i]->data.device().numel();
         size_t j = i + 1;
-        while (j < params_.size() && !covered[j] && !params_[j]->grad.empty() && params_[j]->grad_home.defined() &&
+        // 8-bit moments: a parameter of its own, so that its blocks of 32 start with it
+        while (bits_ == 32 && j < params_.size() && !covered[j] && !params_[j]->grad.empty() && params_[j]->grad_home.defined() &&
                params_[i]->grad_home.defined()) {
             float* pj = params_[j]->data.device().f32();
             float* gj = params_[j]->grad.device().f32();
@@ -275,8 +277,18 @@ void AdamW::build_runs() {
             r.last = j;
             ++j;
         }
-        r.m = Tensor::zeros(1, r.n, DType::F32, device::Pool::Persistent);
-        r.v = Tensor::zeros(1, r.n, DType::F32, device::Pool::Persistent);
+        if (bits_ == 32) {
+            r.m = Tensor::zeros(1, r.n, DType::F32, device::Pool::Persistent);
+            r.v = Tensor::zeros(1, r.n, DType::F32, device::Pool::Persistent);
+        } else {  // zero bytes are moments of zero
+            const size_t nb = (r.n + 31) / 32;
+            r.m = Tensor::bytes(r.n, device::Pool::Persistent);
+            r.v = Tensor::bytes(r.n, device::Pool::Persistent);
+            r.ms = Tensor::bytes(nb, device::Pool::Persistent);
+            r.vs = Tensor::bytes(nb, device::Pool::Persistent);
+            for (const auto& [t, bytes] : {std::pair<Tensor*, size_t>{&r.m, r.n}, {&r.v, r.n}, {&r.ms, nb}, {&r.vs, nb}})
+                check(pk_memset(t->ptr(), 0, bytes, device::stream()), "pk_memset");
+        }
         runs_.push_back(std::move(r));
         // moments imported before this state existed
         const Run& made = runs_.back();
@@ -284,10 +296,7 @@ void AdamW::build_runs() {
             auto it = pending_.find(k);
             if (it == pending_.end()) continue;
             const size_t off = static_cast<size_t>(params_[k]->data.device().f32() - made.p);
-            const size_t bytes = it->second.m.size() * sizeof(float);
-            check(pk_memcpy_h2d(made.m.f32() + off, it->second.m.data(), bytes, device::stream()), "pk_memcpy_h2d");
-            check(pk_memcpy_h2d(made.v.f32() + off, it->second.v.data(), bytes, device::stream()), "pk_memcpy_h2d");
-            device::synchronize();  // the host vectors go away below
+            put_state(made, off, it->second.m.size(), it->second.m.data(), it->second.v.data());
             pending_.erase(it);
         }
         i = j;
@@ -309,8 +318,22 @@ void AdamW::export_state(size_t index, float* m_h, float* v_h) {
     const size_t n = params_[index]->data.rows() * params_[index]->data.cols();
     size_t run = 0, off = 0;
     if (locate(index, &run, &off)) {
-        check(pk_memcpy_d2h(m_h, runs_[run].m.f32() + off, n * sizeof(float), device::stream()), "pk_memcpy_d2h");
-        check(pk_memcpy_d2h(v_h, runs_[run].v.f32() + off, n * sizeof(float), device::stream()), "pk_memcpy_d2h");
+        const Run& r = runs_[run];
+        void* s = device::stream();
+        Tensor m, v;
+        const float *mp = r.m.f32() + off, *vp = r.v.f32() + off;
+        if (bits_ == 8) {
+            m = Tensor::empty(1, n, DType::F32);
+            v = Tensor::empty(1, n, DType::F32);
+            check(pk_adamw_moment_unpack(s, r.m.ptr(), static_cast<const uint8_t*>(r.ms.ptr()), m.f32(), static_cast<int64_t>(n), 0),
+                  "pk_adamw_moment_unpack");
+            check(pk_adamw_moment_unpack(s, r.v.ptr(), static_cast<const uint8_t*>(r.vs.ptr()), v.f32(), static_cast<int64_t>(n), 1),
+                  "pk_adamw_moment_unpack");
+            mp = m.f32();
+            vp = v.f32();
+        }
+        check(pk_memcpy_d2h(m_h, mp, n * sizeof(float), s), "pk_memcpy_d2h");
+        check(pk_memcpy_d2h(v_h, vp, n * sizeof(float), s), "pk_memcpy_d2h");
         device::synchronize();
         return;
     }
@@ -326,14 +349,87 @@ void AdamW::import_state(size_t index, const float* m_h, const float* v_h) {
     const size_t n = params_[index]->data.rows() * params_[index]->data.cols();
     size_t run = 0, off = 0;
     if (locate(index, &run, &off)) {
-        check(pk_memcpy_h2d(runs_[run].m.f32() + off, m_h, n * sizeof(float), device::stream()), "pk_memcpy_h2d");
-        check(pk_memcpy_h2d(runs_[run].v.f32() + off, v_h, n * sizeof(float), device::stream()), "pk_memcpy_h2d");
-        device::synchronize();
+        put_state(runs_[run], off, n, m_h, v_h);
         return;
     }
     Pending& pd = pending_[index];
     pd.m.assign(m_h, m_h + n);
     pd.v.assign(v_h, v_h + n);
+}
+
+// n moments starting `offset` elements into a run, from the host.
+void AdamW::put_state(const Run& r, size_t offset, size_t n, const float* m_h, const float* v_h) {
+    void* s = device::stream();
+    const size_t bytes = n * sizeof(float);
+    if (bits_ == 32) {
+        check(pk_memcpy_h2d(r.m.f32() + offset, m_h, bytes, s), "pk_memcpy_h2d");
+        check(pk_memcpy_h2d(r.v.f32() + offset, v_h, bytes, s), "pk_memcpy_h2d");
+    } else {  // a run is one parameter: offset is 0
+        Tensor m = Tensor::empty(1, n, DType::F32), v = Tensor::empty(1, n, DType::F32);
+        check(pk_memcpy_h2d(m.ptr(), m_h, bytes, s), "pk_memcpy_h2d");
+        check(pk_memcpy_h2d(v.ptr(), v_h, bytes, s), "pk_memcpy_h2d");
+        check(pk_adamw_moment_pack(s, m.f32(), r.m.ptr(), static_cast<uint8_t*>(r.ms.ptr()), static_cast<int64_t>(n), 0), "pk_adamw_moment_pack");
+        check(pk_adamw_moment_pack(s, v.f32(), r.v.ptr(), static_cast<uint8_t*>(r.vs.ptr()), static_cast<int64_t>(n), 1), "pk_adamw_moment_pack");
+    }
+    device::synchronize();  // the host buffers belong to the caller
+}
+
+void AdamW::set_state_bits(int bits) {
+    if (bits != 8 && bits != 32) throw std::runtime_error("AdamW: state bits must be 8 or 32");
+    if (!runs_.empty() && bits != bits_) throw std::runtime_error("AdamW: the moments already exist; set their bits before the first step");
+    bits_ = bits;
+}
+
+void AdamW::set_rates(size_t index, float lr_mult, float weight_decay) {
+    if (index >= params_.size()) throw std::runtime_error("AdamW: parameter index out of range");
+    rates_[index] = {lr_mult, weight_decay};
+}
+
+void* AdamW::plan() {
+    std::vector<pk_adamw_tensor> tensors;
+    std::vector<std::vector<uint64_t>> key;
+    auto add = [&](const Run& r, size_t off, size_t n, float* p, const float* g, void* shadow, Rates rate) {
+        pk_adamw_tensor t{};
+        t.p = p;
+        t.g = g;
+        if (bits_ == 32) {
+            t.m = r.m.f32() + off;
+            t.v = r.v.f32() + off;
+        } else {
+            t.m = r.m.ptr();
+            t.v = r.v.ptr();
+            t.m_scale = static_cast<uint8_t*>(r.ms.ptr());
+            t.v_scale = static_cast<uint8_t*>(r.vs.ptr());
+        }
+        t.shadow = shadow;
+        t.n = static_cast<int64_t>(n);
+        t.lr_mult = rate.lr_mult;
+        t.weight_decay = rate.weight_decay;
+        tensors.push_back(t);
+        uint32_t rb[2];
+        std::memcpy(rb, &rate, sizeof(rb));
+        key.push_back({reinterpret_cast<uint64_t>(p), reinterpret_cast<uint64_t>(g), reinterpret_cast<uint64_t>(t.m),
+                       reinterpret_cast<uint64_t>(shadow), n, (static_cast<uint64_t>(rb[0]) << 32) | rb[1]});
+    };
+    for (const Run& r : runs_) {
+        if (rates_.empty()) {
+            add(r, 0, r.n, r.p, r.g, r.shadow, {1.0f, wd_});
+            continue;
+        }
+        for (size_t i = r.first; i <= r.last; ++i) {
+            const size_t off = static_cast<size_t>(params_[i]->data.device().f32() - r.p);
+            auto it = rates_.find(i);
+            add(r, off, params_[i]->data.device().numel(), r.p + off, r.g + off,
+                r.shadow ? static_cast<char*>(r.shadow) + 2 * off : nullptr, it == rates_.end() ? Rates{1.0f, wd_} : it->second);
+        }
+    }
+    if (!plan_ || key != planned_) {
+        void* made = nullptr;
+        check(pk_adamw_plan_create(tensors.data(), static_cast<int>(tensors.size()), PK_F32, bits_, &made), "pk_adamw_plan_create");
+        plan_ = std::shared_ptr<void>(made, [](void* h) { pk_adamw_plan_destroy(h); });
+        planned_ = std::move(key);
+    }
+    return plan_.get();
 }
 
 void AdamW::step() {
@@ -342,15 +438,24 @@ void AdamW::step() {
     const float c2 = 1.0f - std::pow(b2_, static_cast<float>(t_));
     build_runs();
     void* s = device::stream();
-    for (auto& r : runs_) {
-        check(pk_adamw(s, r.p, r.g, r.m.f32(), r.v.f32(), static_cast<int64_t>(r.n), lr, b1_, b2_, eps_, wd_, c1, c2,
-                       r.shadow),
-              "pk_adamw");
+    for (auto& r : runs_) {  // a gradient without a home in a flat buffer may have moved since
+        const Var& p = params_[r.first];
+        if (!p->grad_home.defined() && !p->grad.empty()) r.g = p->grad.device().f32();
+    }
+    // One launch for all runs. A single run of 32-bit moments with one set of rates (packed models) needs no plan;
+    // the bits are the same either way.
+    if (bits_ == 32 && rates_.empty() && runs_.size() <= 1) {
+        for (auto& r : runs_)
+            check(pk_adamw(s, r.p, r.g, r.m.f32(), r.v.f32(), static_cast<int64_t>(r.n), lr, b1_, b2_, eps_, wd_, c1, c2, r.shadow),
+                  "pk_adamw");
+    } else if (!runs_.empty()) {
+        check(pk_adamw_multi(s, plan(), lr, b1_, b2_, eps_, c1, c2, static_cast<uint64_t>(t_)), "pk_adamw_multi");
+    }
+    for (auto& r : runs_)
         for (size_t i = r.first; i <= r.last; ++i) {
             params_[i]->data.mark_device_modified();
             if (r.shadow) params_[i]->shadow_version = params_[i]->data.version();
         }
-    }
 }
 void AdamW::zero_grad() { microtorch::zero_grad(params_); }
 

@@ -835,6 +835,108 @@ Var cross_entropy(const Var& logits, const std::vector<int>& targets) {
     });
 }
 
+namespace {
+
+// The vocabulary projection of h by chunks of rows, so that the [rows, vocab] logits never exist as a
+// whole: loss(logits, first row, rows) turns a chunk's logits into their gradient in place, which is
+// at once contracted into dh and dW (fp32, chunks in ascending order).
+struct HeadChunks {
+    const Var& h;
+    const Var& W;
+    bool transposed_w;
+    size_t R, d, V, chunk;
+    bool want_h, want_w;
+    Tensor dh, dw;
+
+    HeadChunks(const Var& h_, const Var& W_, bool transposed, size_t chunk_rows)
+        : h(h_), W(W_), transposed_w(transposed), R(h_->data.rows()), d(h_->data.cols()),
+          V(transposed ? W_->data.rows() : W_->data.cols()), chunk(chunk_rows ? chunk_rows : 16384),
+          want_h(grad_enabled() && h_->requires_grad), want_w(grad_enabled() && W_->requires_grad) {
+        if (d != (transposed ? W->data.cols() : W->data.rows())) throw std::runtime_error("matmul: inner dimensions disagree");
+    }
+    bool want() const { return want_h || want_w; }
+    size_t ld() const { return cdt() == DType::BF16 ? (V + 7) / 8 * 8 : V; }
+    Tensor logits(size_t r0, size_t rc) const {
+        Tensor hc = h->compute().view(r0 * d, rc, d);
+        Tensor out = Tensor::empty_strided(rc, V, ld(), cdt());
+        gemm(hc, false, W->compute(), transposed_w, out, false);
+        return out;
+    }
+    void start_gradients() {
+        if (want_h) dh = new_act(R, d);
+        if (want_w) dw = Tensor::zeros(W->data.rows(), W->data.cols(), DType::F32);
+    }
+    void contract(const Tensor& dlogits, size_t r0, size_t rc) {
+        Tensor hc = h->compute().view(r0 * d, rc, d);
+        const Tensor& wt = W->compute();
+        if (want_h) {  // dh = dlogits W^T   ([in,out] storage)  or  dlogits W   ([out,in] storage)
+            Tensor dhc = dh.view(r0 * d, rc, d);
+            gemm(dlogits, false, wt, !transposed_w, dhc, false);
+        }
+        if (want_w) {
+            if (!transposed_w) gemm(hc, true, dlogits, false, dw, true);   // [in,out] += h^T dlogits
+            else gemm(dlogits, true, hc, false, dw, true);                  // [out,in] += dlogits^T h
+        }
+    }
+    // Node of a scalar whose gradients by h and W are dh and dw.
+    Var node(Tensor out) {
+        Tensor dh_ = dh, dw_ = dw;
+        return record(std::move(out), {h, W}, [dh_, dw_](Variable* self) {
+            const Var& h = self->parents[0];
+            const Var& W = self->parents[1];
+            const float g = self->grad.host()(0, 0);
+            if (h->requires_grad && dh_.defined()) {
+                Tensor t = dh_;
+                if (g != 1.0f) check(pk_scale(S(), t.dt(), t.ptr(), g, t.ptr(), i64(t.numel())), "pk_scale");
+                h->accumulate(t);
+            }
+            if (W->requires_grad && dw_.defined()) {
+                if (W->grad_dtype() == DType::F32) {
+                    Tensor& gw = W->grad_for_accumulate();
+                    check(pk_axpy(S(), gw.dt(), gw.ptr(), dw_.dt(), dw_.ptr(), g, i64(dw_.numel())), "pk_axpy");
+                } else {
+                    Tensor t = dw_;
+                    if (g != 1.0f) check(pk_scale(S(), t.dt(), t.ptr(), g, t.ptr(), i64(t.numel())), "pk_scale");
+                    W->accumulate(t);
+                }
+            }
+        });
+    }
+};
+
+// [1,1] fp32 = sum of rows / denom
+Tensor sum_over(const Tensor& rows, size_t n, double denom) {
+    Tensor sum = Tensor::bytes(8), scratch = Tensor::bytes(pk_reduce_scratch_bytes());
+    check(pk_reduce_sum_f64(S(), rows.f32(), i64(n), 0, 0, static_cast<double*>(sum.ptr()), scratch.ptr()), "pk_reduce_sum_f64");
+    Tensor out = Tensor::empty(1, 1, DType::F32);
+    check(pk_sum_to_mean(S(), static_cast<const double*>(sum.ptr()), denom, out.f32()), "pk_sum_to_mean");
+    return out;
+}
+
+// Optional fp32 row values on the device; an empty vector stays a null pointer.
+Tensor row_values(const std::vector<float>& v, size_t R, const char* what) {
+    if (v.empty()) return Tensor();
+    if (v.size() != R) throw std::runtime_error(std::string(what) + ": one value per row");
+    Matrix m(1, R);
+    std::memcpy(m.data(), v.data(), R * sizeof(float));
+    return Tensor::from_host(m);
+}
+const float* row_ptr(const Tensor& t, size_t r0) { return t.defined() ? t.f32() + r0 : nullptr; }
+void read_rows(const Tensor& t, std::vector<float>* out) {
+    if (!out) return;
+    Matrix m = t.to_host();
+    out->assign(m.data(), m.data() + m.rows() * m.cols());
+}
+// Targets of rows that count; the others may hold anything (-100 is usual).
+void check_targets(const std::vector<int>& targets, const std::vector<float>& weight, size_t R, size_t V) {
+    if (targets.size() != R) throw std::runtime_error("one target per row");
+    for (size_t i = 0; i < R; ++i)
+        if ((weight.empty() || weight[i] != 0.0f) && (targets[i] < 0 || static_cast<size_t>(targets[i]) >= V))
+            throw std::runtime_error("target out of range");
+}
+
+}  // namespace
+
 // cross_entropy(linear(h, W), targets) without ever holding the [rows, vocab] logits: the rows
 // are processed in chunks; each chunk's logits are produced, turned into (softmax - onehot)/R
 // in place, and immediately contracted into dh and dW. Same arithmetic per row as the two
@@ -842,65 +944,114 @@ Var cross_entropy(const Var& logits, const std::vector<int>& targets) {
 // visited differs, and dW sums chunk contributions in ascending chunk order.
 Var linear_cross_entropy(const Var& h, const Var& W, bool transposed_w, const std::vector<int>& targets,
                          size_t chunk_rows) {
-    const size_t R = h->data.rows(), d = h->data.cols();
-    const size_t in = transposed_w ? W->data.cols() : W->data.rows();
-    const size_t V = transposed_w ? W->data.rows() : W->data.cols();
-    if (d != in) throw std::runtime_error("matmul: inner dimensions disagree");
+    HeadChunks head(h, W, transposed_w, chunk_rows);
+    const size_t R = head.R, V = head.V;
     if (targets.size() != R) throw std::runtime_error("cross_entropy: one target per row");
     for (int t : targets)
         if (t < 0 || static_cast<size_t>(t) >= V) throw std::runtime_error("cross_entropy: target out of range");
-    if (chunk_rows == 0) chunk_rows = 16384;
-    const Tensor& ht = h->compute();
-    const Tensor& wt = W->compute();
     Tensor dtg = device_ints(targets);
-    const bool want_h = grad_enabled() && h->requires_grad, want_w = grad_enabled() && W->requires_grad;
-    const bool want = want_h || want_w;
     Tensor rows = Tensor::empty(1, R, DType::F32);
-    Tensor dh, dw;
-    if (want_h) dh = new_act(R, d);
-    if (want_w) dw = Tensor::zeros(W->data.rows(), W->data.cols(), DType::F32);
-    const size_t ldl = cdt() == DType::BF16 ? (V + 7) / 8 * 8 : V;
-    for (size_t r0 = 0; r0 < R; r0 += chunk_rows) {
-        const size_t rc = std::min(chunk_rows, R - r0);
-        Tensor hc = ht.view(r0 * d, rc, d);
-        Tensor logits = Tensor::empty_strided(rc, V, ldl, cdt());
-        gemm(hc, false, wt, transposed_w, logits, false);
-        check(pk_cross_entropy(S(), logits.dt(), logits.ptr(), i64(ldl), static_cast<const int32_t*>(dtg.ptr()) + r0,
-                               rows.f32() + r0, i64(rc), i64(V), 1.0f / static_cast<float>(R), want ? 1 : 0, nullptr),
+    head.start_gradients();
+    for (size_t r0 = 0; r0 < R; r0 += head.chunk) {
+        const size_t rc = std::min(head.chunk, R - r0);
+        Tensor logits = head.logits(r0, rc);
+        check(pk_cross_entropy(S(), logits.dt(), logits.ptr(), i64(head.ld()), static_cast<const int32_t*>(dtg.ptr()) + r0,
+                               rows.f32() + r0, i64(rc), i64(V), 1.0f / static_cast<float>(R), head.want() ? 1 : 0, nullptr),
               "pk_cross_entropy");
-        if (want_h) {  // dh = dlogits W^T   ([in,out] storage)  or  dlogits W   ([out,in] storage)
-            Tensor dhc = dh.view(r0 * d, rc, d);
-            gemm(logits, false, wt, !transposed_w, dhc, false);
-        }
-        if (want_w) {
-            if (!transposed_w) gemm(hc, true, logits, false, dw, true);   // [in,out] += h^T dlogits
-            else gemm(logits, true, hc, false, dw, true);                  // [out,in] += dlogits^T h
+        head.contract(logits, r0, rc);
+    }
+    return head.node(sum_over(rows, R, static_cast<double>(R)));
+}
+
+std::vector<float> linear_token_logprob(const Var& h, const Var& W, bool transposed_w, const std::vector<int>& targets,
+                                        const std::vector<float>& weight, size_t chunk_rows) {
+    NoGrad ng;
+    HeadChunks head(h, W, transposed_w, chunk_rows);
+    check_targets(targets, weight, head.R, head.V);
+    Tensor dtg = device_ints(targets), w = row_values(weight, head.R, "token_logprob");
+    Tensor logp = Tensor::empty(1, head.R, DType::F32), lse = Tensor::empty(1, head.R, DType::F32);
+    for (size_t r0 = 0; r0 < head.R; r0 += head.chunk) {
+        const size_t rc = std::min(head.chunk, head.R - r0);
+        Tensor logits = head.logits(r0, rc);
+        check(pk_token_logprob(S(), logits.dt(), logits.ptr(), i64(head.ld()), static_cast<const int32_t*>(dtg.ptr()) + r0,
+                               row_ptr(w, r0), logp.f32() + r0, lse.f32() + r0, i64(rc), i64(head.V), nullptr),
+              "pk_token_logprob");
+    }
+    std::vector<float> out;
+    read_rows(logp, &out);
+    return out;
+}
+
+Var linear_policy_loss(const Var& h, const Var& W, bool transposed_w, const std::vector<int>& targets, const PolicyTerms& terms,
+                       size_t chunk_rows, std::vector<float>* logp_out, std::vector<float>* kl_out) {
+    HeadChunks head(h, W, transposed_w, chunk_rows);
+    const size_t R = head.R;
+    check_targets(targets, terms.weight, R, head.V);
+    if (terms.advantage.size() != R) throw std::runtime_error("policy_loss: one advantage per row");
+    Tensor dtg = device_ints(targets);
+    Tensor old_logp = row_values(terms.old_logp, R, "policy_loss"), ref = row_values(terms.ref_logp, R, "policy_loss");
+    Tensor adv = row_values(terms.advantage, R, "policy_loss"), weight = row_values(terms.weight, R, "policy_loss");
+    Tensor rows = Tensor::empty(1, R, DType::F32), logp = Tensor::empty(1, R, DType::F32), kl = Tensor::empty(1, R, DType::F32);
+    head.start_gradients();
+    for (size_t r0 = 0; r0 < R; r0 += head.chunk) {
+        const size_t rc = std::min(head.chunk, R - r0);
+        Tensor logits = head.logits(r0, rc);
+        check(pk_policy_loss(S(), logits.dt(), logits.ptr(), i64(head.ld()), static_cast<const int32_t*>(dtg.ptr()) + r0,
+                             row_ptr(old_logp, r0), row_ptr(ref, r0), row_ptr(adv, r0), row_ptr(weight, r0), terms.clip_lo,
+                             terms.clip_hi, terms.kl_coef, 1.0f, rows.f32() + r0, logp.f32() + r0, kl.f32() + r0,
+                             head.want() ? logits.ptr() : nullptr, i64(head.ld()), i64(rc), i64(head.V), nullptr),
+              "pk_policy_loss");
+        head.contract(logits, r0, rc);
+    }
+    read_rows(logp, logp_out);
+    read_rows(kl, kl_out);
+    return head.node(sum_over(rows, R, 1.0));
+}
+
+// The gradient of a row depends on its whole pair, so the rows are visited twice: for the
+// log-probabilities, and for the gradient of the logits, which are produced anew (one chunk stays).
+Var linear_preference_loss(const Var& h, const Var& W, bool transposed_w, const std::vector<int>& targets, const PreferenceTerms& terms,
+                           size_t chunk_rows, std::vector<float>* loss_out, std::vector<float>* margin_out) {
+    HeadChunks head(h, W, transposed_w, chunk_rows);
+    const size_t R = head.R;
+    check_targets(targets, terms.weight, R, head.V);
+    if (terms.seq.size() < 3 || terms.seq.size() % 2 == 0) throw std::runtime_error("preference_loss: 2 n + 1 offsets for n pairs");
+    for (size_t i = 0; i < terms.seq.size(); ++i)
+        if (terms.seq[i] < (i ? terms.seq[i - 1] : 0) || static_cast<size_t>(terms.seq[i]) > R)
+            throw std::runtime_error("preference_loss: offsets must ascend within the rows");
+    const size_t P = terms.seq.size() / 2;
+    Tensor dtg = device_ints(targets), seq = device_ints(terms.seq);
+    Tensor ref = row_values(terms.ref_logp, R, "preference_loss"), weight = row_values(terms.weight, R, "preference_loss");
+    Tensor logp = Tensor::empty(1, R, DType::F32), lse = Tensor::empty(1, R, DType::F32);
+    Tensor dlogp = Tensor::zeros(1, R, DType::F32);  // rows outside every sequence keep a gradient of zero
+    Tensor pair = Tensor::empty(1, P, DType::F32), margin = Tensor::empty(1, P, DType::F32);
+    Tensor kept;
+    for (size_t r0 = 0; r0 < R; r0 += head.chunk) {
+        const size_t rc = std::min(head.chunk, R - r0);
+        Tensor logits = head.logits(r0, rc);
+        check(pk_token_logprob(S(), logits.dt(), logits.ptr(), i64(head.ld()), static_cast<const int32_t*>(dtg.ptr()) + r0,
+                               row_ptr(weight, r0), logp.f32() + r0, lse.f32() + r0, i64(rc), i64(head.V), nullptr),
+              "pk_token_logprob");
+        if (rc == R) kept = logits;
+    }
+    check(pk_preference_loss(S(), logp.f32(), row_ptr(ref, 0), row_ptr(weight, 0), static_cast<const int32_t*>(seq.ptr()), i64(P), i64(R),
+                             terms.beta, terms.label_smoothing, 1.0f / static_cast<float>(P), pair.f32(), margin.f32(),
+                             head.want() ? dlogp.f32() : nullptr, nullptr),
+          "pk_preference_loss");
+    if (head.want()) {
+        head.start_gradients();
+        for (size_t r0 = 0; r0 < R; r0 += head.chunk) {
+            const size_t rc = std::min(head.chunk, R - r0);
+            Tensor logits = kept.defined() ? kept : head.logits(r0, rc);
+            check(pk_token_logprob_bwd(S(), logits.dt(), logits.ptr(), i64(head.ld()), static_cast<const int32_t*>(dtg.ptr()) + r0,
+                                       lse.f32() + r0, dlogp.f32() + r0, logits.ptr(), i64(head.ld()), i64(rc), i64(head.V), nullptr),
+                  "pk_token_logprob_bwd");
+            head.contract(logits, r0, rc);
         }
     }
-    Tensor sum = Tensor::bytes(8), scratch = Tensor::bytes(pk_reduce_scratch_bytes());
-    check(pk_reduce_sum_f64(S(), rows.f32(), i64(R), 0, 0, static_cast<double*>(sum.ptr()), scratch.ptr()), "pk_reduce_sum_f64");
-    Tensor out = Tensor::empty(1, 1, DType::F32);
-    check(pk_sum_to_mean(S(), static_cast<const double*>(sum.ptr()), static_cast<double>(R), out.f32()), "pk_sum_to_mean");
-    return record(std::move(out), {h, W}, [dh, dw](Variable* self) {
-        const Var& h = self->parents[0];
-        const Var& W = self->parents[1];
-        const float g = self->grad.host()(0, 0);
-        if (h->requires_grad && dh.defined()) {
-            Tensor t = dh;
-            if (g != 1.0f) check(pk_scale(S(), t.dt(), t.ptr(), g, t.ptr(), i64(t.numel())), "pk_scale");
-            h->accumulate(t);
-        }
-        if (W->requires_grad && dw.defined()) {
-            if (W->grad_dtype() == DType::F32) {
-                Tensor& gw = W->grad_for_accumulate();
-                check(pk_axpy(S(), gw.dt(), gw.ptr(), dw.dt(), dw.ptr(), g, i64(dw.numel())), "pk_axpy");
-            } else {
-                Tensor t = dw;
-                if (g != 1.0f) check(pk_scale(S(), t.dt(), t.ptr(), g, t.ptr(), i64(t.numel())), "pk_scale");
-                W->accumulate(t);
-            }
-        }
-    });
+    read_rows(pair, loss_out);
+    read_rows(margin, margin_out);
+    return head.node(sum_over(pair, P, static_cast<double>(P)));
 }
 
 // reference: src/ops.cpp:481-537 (first head of q and of k only)
@@ -954,6 +1105,87 @@ Var attention_packed(const Var& qkv, size_t n_heads, size_t seq_len, bool causal
 Var attention(const Var& q, const Var& k, const Var& v, size_t n_heads, size_t n_kv_heads, size_t seq_len,
               bool causal) {
     return attention_impl(q, k, v, n_heads, n_kv_heads, 0.0f, seq_len, causal, false);
+}
+
+// One node: the heads' norm and rotation (pk_qk_norm_rope_fwd), then attention over the results. Its
+// backward takes the gradients of the normed heads from the attention kernels and turns them into those
+// of the projections in place.
+Var attention_qk_norm(const Var& q, const Var& k, const Var& v, const Var& wq, const Var& wk, const std::vector<int>& pos,
+                      float theta_base, size_t rot_q, size_t rot_k, size_t Hq, size_t Hkv, size_t seq_len, bool causal, float eps) {
+    const size_t T = q->data.rows();
+    if (k->data.rows() != T || v->data.rows() != T || Hq == 0 || Hkv == 0 || Hq % Hkv != 0 || q->data.cols() % Hq != 0)
+        throw std::runtime_error("attention_qk_norm: shape mismatch");
+    const size_t dk = q->data.cols() / Hq;
+    if (k->data.cols() != Hkv * dk || v->data.cols() != Hkv * dk) throw std::runtime_error("attention_qk_norm: shape mismatch");
+    if (wq->data.rows() != 1 || wq->data.cols() != dk || wk->data.rows() != 1 || wk->data.cols() != dk)
+        throw std::runtime_error("attention_qk_norm: gains must be [1, head_dim]");
+    if (dk % 2 != 0 || rot_q > Hq || rot_k > Hkv) throw std::runtime_error("attention_qk_norm: bad rotation");
+    if (pos.size() != T) throw std::runtime_error("attention_qk_norm: one position per row");
+    const size_t sl = seq_len == 0 ? T : seq_len;
+    if (sl == 0 || T % sl != 0) throw std::runtime_error("attention_qk_norm: rows not a multiple of seq_len");
+    const size_t B = T / sl;
+    const float scale = 1.0f / std::sqrt(static_cast<float>(dk));
+    const bool turns = rot_q + rot_k > 0;
+    Tensor table, dpos;
+    if (turns) detail::rope_operands(pos, theta_base, dk, table, dpos);
+    const Tensor& qt = q->compute();
+    const Tensor& kt = k->compute();
+    const Tensor& vt = v->compute();
+    Tensor gq = f32_of(wq), gk = f32_of(wk);
+    Tensor qn = new_act(T, Hq * dk), kn = new_act(T, Hkv * dk), out = new_act(T, Hq * dk), lse = Tensor::empty(T, Hq, DType::F32);
+    check(pk_qk_norm_rope_fwd(S(), qt.dt(), qt.ptr(), i64(qt.ld()), kt.ptr(), i64(kt.ld()), gq.f32(), gk.f32(), qn.ptr(),
+                              i64(qn.ld()), kn.ptr(), i64(kn.ld()), i64(T), static_cast<int>(Hq), static_cast<int>(Hkv),
+                              static_cast<int>(dk), static_cast<int>(rot_q), static_cast<int>(rot_k), eps,
+                              turns ? static_cast<const int32_t*>(dpos.ptr()) : nullptr, turns ? table.f32() : nullptr,
+                              turns ? i64(table.rows()) : 0),
+          "pk_qk_norm_rope_fwd");
+    check(pk_attn_fwd(S(), qn.dt(), qn.ptr(), i64(qn.ld()), kn.ptr(), i64(kn.ld()), vt.ptr(), i64(vt.ld()), out.ptr(),
+                      i64(out.ld()), lse.f32(), i64(B), i64(sl), static_cast<int>(Hq), static_cast<int>(Hkv),
+                      static_cast<int>(dk), scale, causal ? 1 : 0),
+          "pk_attn_fwd");
+    Tensor out_saved = out;
+    return record(std::move(out), {q, k, v, wq, wk},
+                  [out_saved, lse, qn, kn, table, dpos, turns, B, sl, Hq, Hkv, dk, rot_q, rot_k, scale, causal, eps](Variable* self) {
+        const Var &q = self->parents[0], &k = self->parents[1], &v = self->parents[2], &wq = self->parents[3], &wk = self->parents[4];
+        const Tensor& qt = q->compute();
+        const Tensor& kt = k->compute();
+        const Tensor& vt = v->compute();
+        const size_t T = qt.rows();
+        Tensor g = grad_of(self);
+        Tensor dq = new_act(T, Hq * dk), dk_ = new_act(T, Hkv * dk), dv = new_act(T, Hkv * dk);
+        {
+            Tensor scratch = Tensor::bytes(pk_attn_bwd_scratch_bytes(i64(B), i64(sl), static_cast<int>(Hq)));
+            check(pk_attn_bwd(S(), qn.dt(), qn.ptr(), i64(qn.ld()), kn.ptr(), i64(kn.ld()), vt.ptr(), i64(vt.ld()), out_saved.ptr(),
+                              i64(out_saved.ld()), lse.f32(), g.ptr(), i64(g.ld()), dq.ptr(), i64(dq.ld()), dk_.ptr(), i64(dk_.ld()),
+                              dv.ptr(), i64(dv.ld()), scratch.ptr(), i64(B), i64(sl), static_cast<int>(Hq), static_cast<int>(Hkv),
+                              static_cast<int>(dk), scale, causal ? 1 : 0),
+                  "pk_attn_bwd");
+        }
+        if (v->requires_grad) v->accumulate(dv);
+        if (!q->requires_grad && !k->requires_grad && !wq->requires_grad && !wk->requires_grad) return;
+        Tensor gq = f32_of(wq), gk = f32_of(wk), tq, tk, scratch;
+        auto gain_grad = [dk](const Var& w, Tensor& tmp) -> float* {  // fp32, accumulated in place when the gradient is
+            if (!w->requires_grad) return nullptr;
+            if (w->grad_dtype() == DType::F32) return w->grad_for_accumulate().f32();
+            tmp = Tensor::zeros(1, dk, DType::F32);
+            return tmp.f32();
+        };
+        float* pq = gain_grad(wq, tq);
+        float* pk = gain_grad(wk, tk);
+        if (pq || pk)
+            scratch = Tensor::bytes(pk_qk_norm_rope_bwd_scratch_bytes(i64(T), static_cast<int>(Hq), static_cast<int>(Hkv), static_cast<int>(dk)));
+        check(pk_qk_norm_rope_bwd(S(), qt.dt(), dq.ptr(), i64(dq.ld()), dk_.ptr(), i64(dk_.ld()), qt.ptr(), i64(qt.ld()), kt.ptr(),
+                                  i64(kt.ld()), gq.f32(), gk.f32(), dq.ptr(), i64(dq.ld()), dk_.ptr(), i64(dk_.ld()), pq, pk,
+                                  scratch.defined() ? scratch.ptr() : nullptr, i64(T), static_cast<int>(Hq), static_cast<int>(Hkv),
+                                  static_cast<int>(dk), static_cast<int>(rot_q), static_cast<int>(rot_k), eps,
+                                  turns ? static_cast<const int32_t*>(dpos.ptr()) : nullptr, turns ? table.f32() : nullptr,
+                                  turns ? i64(table.rows()) : 0),
+              "pk_qk_norm_rope_bwd");
+        if (tq.defined()) wq->accumulate(tq);
+        if (tk.defined()) wk->accumulate(tk);
+        if (q->requires_grad) q->accumulate(dq);
+        if (k->requires_grad) k->accumulate(dk_);
+    });
 }
 
 // reference: src/ops.cpp:1046-1064 (sum of squares in double)

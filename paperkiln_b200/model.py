@@ -199,6 +199,58 @@ class Model:
                                      loss_scale, 1, ctypes.byref(loss)), "mt_model_step")
         return float(loss.value)
 
+    # ---- preference / policy tuning ----
+    @staticmethod
+    def _rows(v, n, dtype=np.float32):
+        if v is None:
+            return None, None
+        v = np.ascontiguousarray(v, dtype=dtype).reshape(-1)
+        if v.size != n:
+            raise ValueError(f"expected {n} values, got {v.size}")
+        return v, v.ctypes.data_as(ctypes.c_void_p)
+
+    def token_logprob(self, ids, targets, seq_len: int = 0, weight=None) -> np.ndarray:
+        """Log-probability of every row's target, no gradient (rows of weight 0: 0)."""
+        ids = np.ascontiguousarray(ids, dtype=np.int32)
+        targets, tp = self._rows(targets, ids.size, np.int32)
+        weight, wp = self._rows(weight, ids.size)
+        out = np.empty(ids.size, dtype=np.float32)
+        _check(libmt().mt_model_token_logprob(self._h, ids.ctypes.data_as(ctypes.c_void_p), tp, wp, ids.size, seq_len,
+                                              out.ctypes.data_as(ctypes.c_void_p)), "mt_model_token_logprob")
+        return out
+
+    def policy_step(self, ids, targets, advantage, seq_len: int = 0, old_logp=None, ref_logp=None, weight=None, clip_lo=0.2,
+                    clip_hi=0.2, kl_coef=0.0, loss_scale=1.0, backward=True) -> dict:
+        """Clipped policy loss with a KL term: {"loss", "logp", "kl"}; gradients as after step()."""
+        ids = np.ascontiguousarray(ids, dtype=np.int32)
+        n = ids.size
+        targets, tp = self._rows(targets, n, np.int32)
+        (old_logp, op), (ref_logp, rp), (advantage, ap), (weight, wp) = (self._rows(v, n) for v in (old_logp, ref_logp, advantage, weight))
+        loss, logp, kl = ctypes.c_float(0.0), np.empty(n, np.float32), np.empty(n, np.float32)
+        _check(libmt().mt_model_policy_step(self._h, ids.ctypes.data_as(ctypes.c_void_p), tp, n, seq_len, op, rp, ap, wp, clip_lo,
+                                            clip_hi, kl_coef, loss_scale, int(backward), ctypes.byref(loss),
+                                            logp.ctypes.data_as(ctypes.c_void_p), kl.ctypes.data_as(ctypes.c_void_p)),
+               "mt_model_policy_step")
+        return {"loss": float(loss.value), "logp": logp, "kl": kl}
+
+    def preference_step(self, ids, targets, seq, seq_len: int = 0, ref_logp=None, weight=None, beta=0.1, label_smoothing=0.0,
+                        loss_scale=1.0, backward=True) -> dict:
+        """Paired log-ratio loss: {"loss", "pair_loss", "margin"}; seq: 2 n + 1 row offsets, chosen and rejected in turn."""
+        ids = np.ascontiguousarray(ids, dtype=np.int32)
+        n = ids.size
+        seq = np.ascontiguousarray(seq, dtype=np.int32).reshape(-1)
+        pairs = (seq.size - 1) // 2
+        if seq.size != 2 * pairs + 1 or pairs < 1:
+            raise ValueError("seq holds 2 n + 1 offsets")
+        targets, tp = self._rows(targets, n, np.int32)
+        (ref_logp, rp), (weight, wp) = (self._rows(v, n) for v in (ref_logp, weight))
+        loss, pair, margin = ctypes.c_float(0.0), np.empty(pairs, np.float32), np.empty(pairs, np.float32)
+        _check(libmt().mt_model_preference_step(self._h, ids.ctypes.data_as(ctypes.c_void_p), tp, n, seq_len, rp, wp,
+                                                seq.ctypes.data_as(ctypes.c_void_p), pairs, beta, label_smoothing, loss_scale,
+                                                int(backward), ctypes.byref(loss), pair.ctypes.data_as(ctypes.c_void_p),
+                                                margin.ctypes.data_as(ctypes.c_void_p)), "mt_model_preference_step")
+        return {"loss": float(loss.value), "pair_loss": pair, "margin": margin}
+
     def live_after_forward(self) -> int:
         n = ctypes.c_int64(0)
         _check(libmt().mt_model_live_after_forward(self._h, ctypes.byref(n)), "mt_model_live_after_forward")
@@ -206,6 +258,14 @@ class Model:
 
     def set_adamw(self, lr=1e-3, beta1=0.9, beta2=0.999, eps=1e-8, weight_decay=0.01):
         _check(libmt().mt_model_set_adamw(self._h, lr, beta1, beta2, eps, weight_decay), "mt_model_set_adamw")
+
+    def set_adamw_state_bits(self, bits: int):
+        """32 (default) or 8: bits of the stored moments; before the first optimizer step."""
+        _check(libmt().mt_model_set_adamw_state_bits(self._h, int(bits)), "mt_model_set_adamw_state_bits")
+
+    def set_param_rates(self, name: str, lr_mult: float = 1.0, weight_decay: float = 0.0):
+        """Learning-rate factor and weight decay of one parameter from the next step on."""
+        _check(libmt().mt_model_set_param_rates(self._h, self._index[name], lr_mult, weight_decay), "mt_model_set_param_rates")
 
     def optimizer_step(self):
         _check(libmt().mt_model_optimizer_step(self._h), "mt_model_optimizer_step")
