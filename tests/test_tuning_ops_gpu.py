@@ -639,10 +639,10 @@ def test_adamw_plan_refuses_overlaps_and_host_memory(pk):
                 for p, g, m, v in tensors]
         return _capi.AdamwPlan(rows, 0, 32)
 
-    make((0, 1024, 2048, 3072), (256, 1024, 2304, 3328)).close()     # two tensors may read one gradient
+    make((0, 1024, 2048, 2560), (256, 1024, 2304, 2816)).close()     # two tensors may read one gradient
     for second in ((0, 1280, 4096, 5120), (128, 1280, 4096, 5120), (512, 1024 + 252, 1024 + 128, 5120)):
         with pytest.raises(_capi.PkError, match="overlaps"):
-            make((0, 1024, 2048, 3072), second)
+            make((0, 1024, 2048, 2560), second)
     host = torch.zeros(64)
     with pytest.raises(_capi.PkError, match="not in the current GPU"):
         _capi.AdamwPlan([_capi.AdamwTensor(p=host.data_ptr(), g=base, m=base + 1024, v=base + 2048, n=64)], 0, 32)
