@@ -181,33 +181,6 @@ __device__ __forceinline__ void row_zero(T* dx, int64_t V, int64_t tid, int64_t 
 
 template <typename T>
 __global__ void __launch_bounds__(512)
-token_logprob_kernel(const T* __restrict__ logits, int64_t ld, const int32_t* __restrict__ targets,
-                     const float* __restrict__ weight, float* __restrict__ logp, float* __restrict__ lse, int64_t R, int64_t V,
-                     int32_t* status) {
-    __shared__ Stat red[16];
-    for (int64_t row = blockIdx.x; row < R; row += gridDim.x) {
-        if (weight != nullptr && weight[row] == 0.0f) {
-            if (threadIdx.x == 0) {
-                logp[row] = 0.0f;
-                lse[row] = 0.0f;
-            }
-            continue;
-        }
-        const T* x = logits + row * ld;
-        const Stat st = block_stat(row_stat(x, V), red);
-        if (threadIdx.x == 0) {
-            const int64_t t = targets[row];
-            const bool ok = t >= 0 && t < V;
-            if (!ok && status) atomicOr(status, PK_ERR_INDEX);
-            const float ls = logf(st.s);
-            lse[row] = st.m + ls;
-            logp[row] = ok ? to_f32(x[t]) - st.m - ls : 0.0f;
-        }
-    }
-}
-
-template <typename T>
-__global__ void __launch_bounds__(512)
 token_logprob_bwd_kernel(const T* logits, int64_t ld, const int32_t* __restrict__ targets, const float* __restrict__ lse,
                          const float* __restrict__ dlogp, T* dlogits, int64_t ldd, int64_t R, int64_t V, int32_t* status) {
     // gridDim.y blocks share a row. Last rows first: the pass that took the log-probabilities has left them in L2.
@@ -279,6 +252,8 @@ __device__ __forceinline__ void policy_row_out(const PolicyArgs& a, int64_t row)
     if (a.kl) a.kl[row] = 0.0f;
 }
 
+// Loss and gradient of rows too long for a cluster: a CTA sweeps its row twice, the second time through L2
+// where it fits (2048 x 400000 bf16).
 template <typename T>
 __global__ void __launch_bounds__(512)
 policy_loss_kernel(const T* logits, int64_t ld, PolicyArgs a, T* dlogits, int64_t ldd, int64_t R, int64_t V) {
@@ -293,7 +268,7 @@ policy_loss_kernel(const T* logits, int64_t ld, PolicyArgs a, T* dlogits, int64_
                 if (w != 0.0f && a.status) atomicOr(a.status, PK_ERR_INDEX);
                 policy_row_out(a, row);
             }
-            if (dlogits) row_zero(dlogits + row * ldd, V, threadIdx.x, blockDim.x);
+            row_zero(dlogits + row * ldd, V, threadIdx.x, blockDim.x);
             continue;
         }
         const T* x = logits + row * ld;
@@ -305,10 +280,8 @@ policy_loss_kernel(const T* logits, int64_t ld, PolicyArgs a, T* dlogits, int64_
         }
         __syncthreads();
         // a gradient of exactly zero (held back by its bound, no KL term) leaves nothing to read
-        if (dlogits) {
-            if (grad == 0.0f) row_zero(dlogits + row * ldd, V, threadIdx.x, blockDim.x);
-            else row_grad(x, dlogits + row * ldd, V, t, st.m, 1.0f / st.s, grad, threadIdx.x, blockDim.x);
-        }
+        if (grad == 0.0f) row_zero(dlogits + row * ldd, V, threadIdx.x, blockDim.x);
+        else row_grad(x, dlogits + row * ldd, V, t, st.m, 1.0f / st.s, grad, threadIdx.x, blockDim.x);
         __syncthreads();
     }
 }
@@ -842,6 +815,121 @@ stream_kernel(const RowArgs a) {
     }
 }
 
+// Long rows without a gradient: one pass, nothing is kept. A CTA, or a cluster of CTAs when there are few
+// rows, per row; a thread holds FORWARD_K vectors in flight and a running sum of exponentials against a
+// reference that follows its maximum only when that has moved by more than 8 (a term stays below e^8, the
+// rounding of its exponent below 2^-20). Nothing orders the rows: the memory stays busy by what else is
+// resident, eight CTAs to an SM. 8192 x 50257 bf16: 150 us, 5.5 TB/s (the kernel above, which waits for a
+// row before it takes the next: 228; four CTAs of 128 registers 158).
+constexpr int FORWARD_THREADS = 256, FORWARD_WARPS = FORWARD_THREADS / 32, FORWARD_K = 4, FORWARD_PER_SM = 8;
+
+template <typename T, bool POLICY>
+__global__ void __launch_bounds__(FORWARD_THREADS, FORWARD_PER_SM)
+forward_kernel(const RowArgs a) {
+    constexpr int N = RowVec<T>::N, THREADS = FORWARD_THREADS, K = FORWARD_K;
+    __shared__ Stat boxes[CLUSTER_PORTABLE * FORWARD_WARPS];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int C = static_cast<int>(cluster_size()), rank = static_cast<int>(cluster_rank());
+    const int64_t r = blockIdx.x / static_cast<unsigned>(C);
+    const bool writer = rank == 0 && tid == 0;
+    if (a.p.weight != nullptr && a.p.weight[r] == 0.0f) {  // the whole cluster
+        if (writer) {
+            if constexpr (POLICY) {
+                policy_row_out(a.p, r);
+            } else {
+                a.lse[r] = 0.0f;
+                a.p.logp[r] = 0.0f;
+            }
+        }
+        return;
+    }
+    if (C > 1) cluster_arrive();  // nobody writes to a CTA's boxes before it runs
+    const T* x = static_cast<const T*>(a.logits) + r * a.ld;
+    const RowSplit<T> sp(x, a.V);
+    int64_t t = 0;
+    bool ok = false;
+    float xt = 0.0f;
+    PolicyRow q;
+    if (writer) {
+        t = a.p.targets[r];
+        ok = t >= 0 && t < a.V;
+        if constexpr (POLICY) q.load(a.p, r);
+        if (ok) xt = to_f32(x[t]);
+    }
+    float edge = -INFINITY;  // the elements before the first and behind the last vector belong to the first threads
+    if (rank == 0 && tid < sp.head + a.V - sp.tail0) edge = to_f32(x[tid < sp.head ? tid : sp.tail0 + tid - sp.head]);
+
+    const int64_t slice = (sp.nv + C - 1) / C, from = rank * slice, to = min(from + slice, sp.nv);
+    const T* body = x + sp.head;
+    Base base(-INFINITY);
+    float top = -INFINITY, sum = 0.0f;
+    auto follow = [&](float m) {
+        if (m > top + 8.0f) {
+            const Base next(m);
+            if (top != -INFINITY) sum *= ex2((top - next.m) * LOG2E - base.r + next.r);  // else it is 0, or NaN
+            top = m;
+            base = next;
+        }
+    };
+    constexpr uint32_t FILL = sizeof(T) == 2 ? 0xff80ff80u : 0xff800000u;  // -inf
+    for (int64_t i = from + tid; i < to; i += K * THREADS) {
+        uint4 raw[K];
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+            raw[k] = make_uint4(FILL, FILL, FILL, FILL);
+            if (i + k * THREADS < to) raw[k] = Vec<T>::load_raw(body + (i + k * THREADS) * N);
+        }
+        RowVec<T> most;
+#pragma unroll
+        for (int k = 0; k < K; ++k) most.add(raw[k]);
+        follow(most.top(-INFINITY));
+        uint64_t part[2] = {};
+        auto take = [&](auto form) {
+            constexpr bool PLAIN = decltype(form)::value;
+#pragma unroll
+            for (int k = 0; k < K; ++k) {
+                uint64_t p[N / 2];
+                unpack2(raw[k], p);
+#pragma unroll
+                for (int e = 0; e < N / 2; ++e) part[e & 1] = tc::f2_add(part[e & 1], base.template of2<PLAIN>(p[e]));
+            }
+        };
+        if (base.plain) take(std::true_type());
+        else take(std::false_type());
+        float lo, hi;
+        tc::f2_unpack(tc::f2_add(part[0], part[1]), lo, hi);
+        sum += lo + hi;
+    }
+    follow(edge);
+    sum += base.plain ? base.template of<true>(edge) : base.template of<false>(edge);
+    Stat st = warp_stat({top, sum * ex2(-base.r)});
+    if (C == 1) {
+        if (lane == 0) boxes[warp] = st;
+        __syncthreads();
+    } else {
+        cluster_wait();
+        if (lane == 0) cluster_store(tc::smem_u32(&boxes[rank * FORWARD_WARPS + warp]), 0, st);
+        __syncwarp();
+        cluster_arrive();
+        cluster_wait();
+    }
+    if (rank != 0 || warp != 0) return;
+    st = {-INFINITY, 0.0f};
+    for (int k = lane; k < C * FORWARD_WARPS; k += 32) st = merge(st, boxes[k]);
+    st = warp_stat(st);
+    if (!writer) return;
+    const float ls = logf(st.s);
+    if (!ok && a.p.status) atomicOr(a.p.status, PK_ERR_INDEX);
+    if constexpr (!POLICY) {
+        a.lse[r] = st.m + ls;
+        a.p.logp[r] = ok ? xt - st.m - ls : 0.0f;
+    } else if (ok) {
+        policy_row(a.p, r, q, xt - st.m - ls, true);
+    } else {
+        policy_row_out(a.p, r);
+    }
+}
+
 // One block per pair. Sums in fp64: a thread's rows in ascending order, then a fixed tree. A pair is a few
 // thousand rows, so the time is latency: four rows per thread are loaded side by side (12 -> 7 us for four
 // pairs of 2 x 800 rows).
@@ -953,14 +1041,42 @@ void stream_form(const void** kernel, size_t* smem) {
     *smem = Stream<T, POLICY, SLOTS>::SMEM;
 }
 
-// Launches the on-chip kernels; *taken is false when a row does not fit a cluster.
+int launch_clusters(cudaStream_t st, const void* kernel, int64_t ctas, int size, int threads, size_t smem, RowArgs& a) {
+    PK_REQUIRE(ctas <= 0x7fffffff, "too many rows");
+    cudaLaunchConfig_t cfg{};
+    cudaLaunchAttribute at{};
+    at.id = cudaLaunchAttributeClusterDimension;
+    at.val.clusterDim.x = static_cast<unsigned>(size);
+    at.val.clusterDim.y = at.val.clusterDim.z = 1;
+    cfg.gridDim = dim3(static_cast<unsigned>(ctas));
+    cfg.blockDim = dim3(static_cast<unsigned>(threads));
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cfg.attrs = &at;
+    cfg.numAttrs = size > 1 ? 1 : 0;
+    void* args[] = {&a};
+    PK_CHECK_CUDA(cudaLaunchKernelExC(&cfg, kernel, args));
+    return PK_OK;
+}
+
+// Launches the kernels that read the logits once; *taken is false when there is a gradient and a row does
+// not fit a cluster.
 template <typename T, bool POLICY>
 int launch_rows(cudaStream_t st, RowArgs a, bool* taken) {
     constexpr int N = Vec<T>::N, K = RowK<T>::K;
     const int64_t vectors = (a.V + N - 1) / N;
+    const int sms = sm_count();
+    *taken = true;
+    // From 7 vectors per thread on the free-running rows win (16000 x 16000 bf16 101 against 108 us, 24000 x
+    // 10000 133 against 104).
+    if (a.dlogits == nullptr && vectors >= 7 * FORWARD_THREADS) {
+        // few rows: clusters, down to two vectors per thread (100 x 151936 bf16: 27 us with one CTA, 16 with eight)
+        int size = 1;
+        while (size < CLUSTER_PORTABLE && a.R * size * 2 <= sms * 6 && vectors >= static_cast<int64_t>(4) * FORWARD_THREADS * size) size *= 2;
+        return launch_clusters(st, reinterpret_cast<const void*>(forward_kernel<T, POLICY>), a.R * size, size, FORWARD_THREADS, 0, a);
+    }
     *taken = vectors <= static_cast<int64_t>(Stream<T, POLICY, 10>::SLICE) * CLUSTER_MOST;
     if (!*taken) return PK_OK;
-    const int sms = sm_count();
     // the fewest warps that hold a row, and more while that leaves SMs without a row
     int wpr = vectors <= K * 32 ? 1 : (vectors <= K * 128 ? 4 : ROW_WARPS);
     while (wpr < ROW_WARPS && a.R * wpr < static_cast<int64_t>(sms) * 8) wpr *= 4;
@@ -972,9 +1088,14 @@ int launch_rows(cudaStream_t st, RowArgs a, bool* taken) {
         smem = static_cast<size_t>(2) * a.slots * ROW_THREADS * 16;
     } else {
         threads = STREAM_THREADS;
-        // Up to 16384 vectors 8 CTAs hold a row; more CTAs beyond that beat more vectors per thread (2048 x 200064
-        // bf16: 13 CTAs of 8 vectors 414 us, 8 CTAs of 16 vectors at two per SM 512, sweeps 481).
-        while (size < CLUSTER_MOST && vectors > static_cast<int64_t>(Stream<T, POLICY, 8>::SLICE) * size) ++size;
+        // The fewest CTAs of up to 8 vectors per thread: every CTA more makes a row's chain longer (8192 x 50257
+        // bf16: 4 CTAs 387 us, 5 405, 6 479). Seven fill the SMs' groups badly (1021 x 50257 fp32: 100 us, with
+        // eight 92). Beyond eight CTAs 10 vectors per thread, although some of them spill, beat more CTAs (2048 x
+        // 200064 bf16: 10 CTAs 362 us, 13 407; sweeps 481).
+        constexpr int64_t SLICE8 = Stream<T, POLICY, 8>::SLICE, SLICE10 = Stream<T, POLICY, 10>::SLICE;
+        size = static_cast<int>((vectors + SLICE8 - 1) / SLICE8);
+        if (size == 7) size = 8;
+        if (size > 8) size = static_cast<int>((vectors + SLICE10 - 1) / SLICE10);
         // few rows: more CTAs to a row, down to two vectors per thread; beyond 8 CTAs nothing is gained
         while (size < CLUSTER_PORTABLE && a.R * size * 2 <= sms * 4 && vectors >= static_cast<int64_t>(4) * STREAM_THREADS * size)
             size = std::min(size * 2, CLUSTER_PORTABLE);
@@ -983,30 +1104,21 @@ int launch_rows(cudaStream_t st, RowArgs a, bool* taken) {
         else if (slice <= Stream<T, POLICY, 5>::SLICE) stream_form<T, POLICY, 5>(&kernel, &smem);
         else if (slice <= Stream<T, POLICY, 6>::SLICE) stream_form<T, POLICY, 6>(&kernel, &smem);
         else if (slice <= Stream<T, POLICY, 7>::SLICE) stream_form<T, POLICY, 7>(&kernel, &smem);
-        else if (slice <= Stream<T, POLICY, 8>::SLICE) stream_form<T, POLICY, 8>(&kernel, &smem);
-        else stream_form<T, POLICY, 10>(&kernel, &smem);
+        else if constexpr (POLICY) {  // log-probabilities of longer rows are taken above
+            if (slice <= SLICE8) stream_form<T, POLICY, 8>(&kernel, &smem);
+            else stream_form<T, POLICY, 10>(&kernel, &smem);
+        }
         most = smem;
     }
     const int resident = resident_clusters(kernel, size, threads, smem, most);
+    if (resident == 0 && a.dlogits == nullptr)
+        return launch_clusters(st, reinterpret_cast<const void*>(forward_kernel<T, POLICY>), a.R, 1, FORWARD_THREADS, 0, a);
     if (resident == 0) {
         *taken = false;
         return PK_OK;
     }
     const int64_t groups = wpr == ROW_WARPS ? a.R : (a.R + ROW_WARPS / wpr - 1) / (ROW_WARPS / wpr);
-    cudaLaunchConfig_t cfg{};
-    cudaLaunchAttribute at{};
-    at.id = cudaLaunchAttributeClusterDimension;
-    at.val.clusterDim.x = static_cast<unsigned>(size);
-    at.val.clusterDim.y = at.val.clusterDim.z = 1;
-    cfg.gridDim = dim3(static_cast<unsigned>(std::min<int64_t>(groups, resident) * size));
-    cfg.blockDim = dim3(static_cast<unsigned>(threads));
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = st;
-    cfg.attrs = &at;
-    cfg.numAttrs = size > 1 ? 1 : 0;
-    void* args[] = {&a};
-    PK_CHECK_CUDA(cudaLaunchKernelExC(&cfg, kernel, args));
-    return PK_OK;
+    return launch_clusters(st, kernel, std::min<int64_t>(groups, resident) * size, size, threads, smem, a);
 }
 
 // dlogits may be logits itself or must not touch it.
@@ -1034,18 +1146,8 @@ int pk_token_logprob(void* stream, int dtype, const void* logits, int64_t ld, co
     RowArgs a{};
     a.logits = logits; a.ld = ld; a.R = R; a.V = V; a.lse = lse;
     a.p.targets = targets; a.p.weight = weight; a.p.logp = logp; a.p.status = status;
-    bool taken = false;
-    const int rc = dtype == PK_F32 ? launch_rows<float, false>(as_stream(stream), a, &taken) : launch_rows<bf16, false>(as_stream(stream), a, &taken);
-    if (rc != PK_OK || taken) return rc;
-    const int threads = row_threads(V);
-    if (dtype == PK_F32)
-        token_logprob_kernel<float><<<row_blocks(R), threads, 0, as_stream(stream)>>>(
-            static_cast<const float*>(logits), ld, targets, weight, logp, lse, R, V, status);
-    else
-        token_logprob_kernel<bf16><<<row_blocks(R), threads, 0, as_stream(stream)>>>(
-            static_cast<const bf16*>(logits), ld, targets, weight, logp, lse, R, V, status);
-    PK_LAUNCH_CHECK();
-    return PK_OK;
+    bool taken = false;  // always, without a gradient
+    return dtype == PK_F32 ? launch_rows<float, false>(as_stream(stream), a, &taken) : launch_rows<bf16, false>(as_stream(stream), a, &taken);
 }
 
 int pk_token_logprob_bwd(void* stream, int dtype, const void* logits, int64_t ld, const int32_t* targets,
