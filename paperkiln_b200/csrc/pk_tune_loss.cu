@@ -25,6 +25,14 @@ __device__ __forceinline__ float ex2(float x) {
     return y;
 }
 
+// The kernels of this file are launched while their predecessor on the stream still runs, and wait for it here
+// before they touch memory: the cost of a launch is then behind them. The three calls of a paired loss, 2 x 40 rows of
+// 32000 bf16: 21 -> 16 us, 8192 rows 210 -> 204; replayed from a graph, where a launch costs little, 9.4 -> 10.6.
+__device__ __forceinline__ void after_predecessor() {
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+}
+
 // Running maximum and sum of exponentials of a thread's or a row's values. An empty one has
 // m = -inf and s = 0, and so has a row of nothing but -inf.
 struct __align__(8) Stat {
@@ -70,14 +78,13 @@ template <typename T> struct RowSplit {
     }
 };
 
-// dx[j] = g ([j == t] - exp(x_j - base) * inv): `threads` threads, of which this is `tid`, write one row. x
-// and dx may be the same row; they are read and written by the same thread, element by element or vector by vector.
+// dx[j] = g ([j == t] - exp(x_j - lse)): `threads` threads, of which this is `tid`, write one row. x and dx may be
+// the same row; they are read and written by the same thread, element by element or vector by vector.
 template <typename T>
-__device__ __forceinline__ void row_grad(const T* x, T* dx, int64_t V, int64_t t, float base, float inv, float g, int64_t tid, int64_t threads) {
+__device__ __forceinline__ void row_grad(const T* x, T* dx, int64_t V, int64_t t, float lse, float g, int64_t tid, int64_t threads) {
     constexpr int N = Vec<T>::N;
     const RowSplit<T> sp(x, V);
     const bool wide = ((reinterpret_cast<uintptr_t>(x) ^ reinterpret_cast<uintptr_t>(dx)) & 15u) == 0;
-    const float k = -g * inv;
     if (wide) {
         const T* body = x + sp.head;
         T* out = dx + sp.head;
@@ -87,7 +94,7 @@ __device__ __forceinline__ void row_grad(const T* x, T* dx, int64_t V, int64_t t
             const int64_t te = t - sp.head - i * N;
 #pragma unroll
             for (int e = 0; e < N; ++e) {
-                f[e] = ex2((f[e] - base) * LOG2E) * k;
+                f[e] = ex2((f[e] - lse) * LOG2E) * -g;
                 if (te == e) f[e] += g;
             }
             Vec<T>::store(out + i * N, f);
@@ -96,7 +103,7 @@ __device__ __forceinline__ void row_grad(const T* x, T* dx, int64_t V, int64_t t
     const int64_t edge = wide ? sp.head + V - sp.tail0 : V;  // elements outside the vectors
     for (int64_t i = tid; i < edge; i += threads) {
         const int64_t c = !wide || i < sp.head ? i : sp.tail0 + i - sp.head;
-        float f = ex2((to_f32(x[c]) - base) * LOG2E) * k;
+        float f = ex2((to_f32(x[c]) - lse) * LOG2E) * -g;
         if (c == t) f += g;
         dx[c] = from_f32<T>(f);
     }
@@ -116,13 +123,14 @@ token_logprob_bwd_kernel(const T* logits, int64_t ld, const int32_t* __restrict_
                          const float* __restrict__ dlogp, T* dlogits, int64_t ldd, int64_t R, int64_t V, int32_t* status) {
     // gridDim.y blocks share a row. Last rows first: the pass that took the log-probabilities has left them in L2.
     const int64_t tid = blockIdx.y * blockDim.x + threadIdx.x, threads = gridDim.y * blockDim.x;
+    after_predecessor();
     for (int64_t row = R - 1 - blockIdx.x; row >= 0; row -= gridDim.x) {
         float g = dlogp[row];
         T* dx = dlogits + row * ldd;
         if (g != 0.0f) {
             const int64_t t = targets[row];
             if (t >= 0 && t < V) {
-                row_grad(logits + row * ld, dx, V, t, lse[row], 1.0f, g, tid, threads);
+                row_grad(logits + row * ld, dx, V, t, lse[row], g, tid, threads);
                 continue;
             }
             if (tid == 0 && status) atomicOr(status, PK_ERR_INDEX);
@@ -259,6 +267,7 @@ __device__ __forceinline__ uint4 pack(const float (&f)[8]) {
     }
     return make_uint4(w[0], w[1], w[2], w[3]);
 }
+
 // A row belongs to a warp (THREADS = 32, four rows to a CTA), a CTA, or a cluster of 2 to 8 CTAs with a
 // stretch of it each. A thread holds K vectors in flight and a running sum of exponentials against a
 // reference that follows its maximum only when that has moved by more than 8 (a term stays below e^8, the
@@ -277,6 +286,9 @@ template <bool GRAD, int THREADS> struct Sweep {
     static constexpr int PER_SM = GRAD ? (CTA == 128 ? 10 : 6) : 2048 / CTA;
 };
 
+// The second reading is the last, and nobody reads the gradient before the kernel's end: both are marked to
+// leave L2 first, so that they do not push out stretches that have yet to be read again (8192 x 32000 bf16 219 -> 192 us
+// before the second reading went backwards).
 __device__ __forceinline__ uint4 load_last(const void* p) { return __ldcs(static_cast<const uint4*>(p)); }
 
 template <typename T, bool POLICY, bool GRAD, int THREADS>
@@ -290,6 +302,7 @@ sweep_kernel(const RowArgs a) {
     const int tid = threadIdx.x % THREADS, lane = tid & 31, warp = tid >> 5;
     const int C = WARP ? 1 : static_cast<int>(cluster_size()), rank = WARP ? 0 : static_cast<int>(cluster_rank());
     const int64_t r = WARP ? static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 5) : blockIdx.x / static_cast<unsigned>(C);
+    after_predecessor();
     if (WARP && r >= a.R) return;
     const bool writer = rank == 0 && tid == 0;
     T* dx = GRAD ? static_cast<T*>(a.dlogits) + r * a.ldd : nullptr;
@@ -483,6 +496,7 @@ preference_loss_kernel(const float* __restrict__ logp, const float* __restrict__
     __shared__ double red[WARPS];
     __shared__ float dz_s;
     const int64_t pair = blockIdx.x;
+    after_predecessor();
     const int64_t a = seq[2 * pair], b = seq[2 * pair + 1], c = seq[2 * pair + 2];
     if (a < 0 || b < a || c < b || c > R) {
         if (threadIdx.x == 0) {
@@ -542,46 +556,49 @@ preference_loss_kernel(const float* __restrict__ logp, const float* __restrict__
 int row_threads(int64_t V) { return V >= 4096 ? 512 : (V >= 1024 ? 256 : 128); }
 unsigned row_blocks(int64_t R) { return static_cast<unsigned>(std::min<int64_t>(R, static_cast<int64_t>(sm_count()) * 8)); }
 
-int launch_clusters(cudaStream_t st, const void* kernel, int64_t ctas, int size, int threads, RowArgs& a) {
-    PK_REQUIRE(ctas <= 0x7fffffff, "too many rows");
+// A launch in clusters of `size` CTAs (1: none) that may start before its predecessor has ended.
+template <typename... P, typename... A>
+int launch(cudaStream_t st, void (*kernel)(P...), dim3 grid, int size, int threads, const A&... args) {
     cudaLaunchConfig_t cfg{};
-    cudaLaunchAttribute at{};
-    at.id = cudaLaunchAttributeClusterDimension;
-    at.val.clusterDim.x = static_cast<unsigned>(size);
-    at.val.clusterDim.y = at.val.clusterDim.z = 1;
-    cfg.gridDim = dim3(static_cast<unsigned>(ctas));
+    cudaLaunchAttribute at[2] = {};
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    at[1].id = cudaLaunchAttributeClusterDimension;
+    at[1].val.clusterDim.x = static_cast<unsigned>(size);
+    at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
+    cfg.gridDim = grid;
     cfg.blockDim = dim3(static_cast<unsigned>(threads));
     cfg.stream = st;
-    cfg.attrs = &at;
-    cfg.numAttrs = size > 1 ? 1 : 0;
-    void* args[] = {&a};
-    PK_CHECK_CUDA(cudaLaunchKernelExC(&cfg, kernel, args));
+    cfg.attrs = at;
+    cfg.numAttrs = size > 1 ? 2 : 1;
+    PK_CHECK_CUDA(cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...));
     return PK_OK;
 }
 
 template <typename T, bool POLICY, bool GRAD>
-int launch_rows(cudaStream_t st, RowArgs a) {
+int launch_rows(cudaStream_t st, const RowArgs& a) {
     constexpr int N = Vec<T>::N;
     const int64_t vectors = (a.V + N - 1) / N;
     const int sms = sm_count();
-    // Threads per row, us with a gradient in bf16 for 32 / 128 / 256: 32000 x 6000 139 / 164 / 201, 32000 x 8000 188 / 184 / 217,
-    // 16000 x 16000 - / 174 / 180, 12000 x 24000 - / 207 / 197. Few rows take more: 1000 x 3000 12.3 / 10.2 / 14.3,
-    // 400 x 6000 16.4 / 12.3 / 10.2.
+    // Threads per row, us with a gradient in bf16 for 32 / 128 / 256: 32000 x 6000 139 / 164 / 201, 32000 x 8000
+    // 188 / 184 / 217, 16000 x 16000 - / 174 / 180, 12000 x 24000 - / 207 / 197. Few rows take more: 1000 x 3000
+    // 12.3 / 10.2 / 14.3, 400 x 6000 16.4 / 12.3 / 10.2.
     int threads = vectors <= 896 ? 32 : (vectors <= 2048 ? 128 : 256);
     if (threads == 32 && vectors >= 256 && a.R <= sms * 8) threads = 128;
     if (threads == 128 && vectors >= 512 && a.R <= sms * 4) threads = 256;
-    if (threads == 32) return launch_clusters(st, reinterpret_cast<const void*>(sweep_kernel<T, POLICY, GRAD, 32>), (a.R + 3) / 4, 1, 128, a);
+    PK_REQUIRE(a.R <= 0x7fffffff / CLUSTER_MOST, "too many rows");
+    if (threads == 32) return launch(st, sweep_kernel<T, POLICY, GRAD, 32>, dim3(static_cast<unsigned>((a.R + 3) / 4)), 1, 128, a);
     int size = 1;
-    // With a gradient a CTA's stretch is at most 100 KB, so that the stretches of all resident CTAs stay in L2: 2048 x
-    // 151936 bf16 295 us with one CTA per row, 262 with two, 240 with four, 276 with eight.
+    // With a gradient a CTA's stretch is at most 100 KB, so that the stretches of all resident CTAs stay in L2:
+    // 2048 x 151936 bf16 295 us with one CTA per row, 262 with two, 240 with four, 276 with eight.
     if (GRAD)
         while (size < CLUSTER_MOST && vectors > static_cast<int64_t>(6400) * size) size *= 2;
-    // few rows: as many CTAs as are resident, down to two vectors per thread (100 x 151936 bf16 without a gradient: 27 us
-    // with one CTA per row, 16 with eight; 400 rows 39, with two 36, with eight 43)
+    // few rows: as many CTAs as are resident, down to two vectors per thread (100 x 151936 bf16 without a gradient:
+    // 27 us with one CTA per row, 16 with eight; 400 rows 39, with two 36, with eight 43)
     while (size < CLUSTER_MOST && a.R * size * 2 <= sms * 6 && vectors >= static_cast<int64_t>(4) * threads * size) size *= 2;
-    const void* kernel = threads == 128 ? reinterpret_cast<const void*>(sweep_kernel<T, POLICY, GRAD, 128>)
-                                        : reinterpret_cast<const void*>(sweep_kernel<T, POLICY, GRAD, 256>);
-    return launch_clusters(st, kernel, a.R * size, size, threads, a);
+    const dim3 grid(static_cast<unsigned>(a.R * size));
+    return threads == 128 ? launch(st, sweep_kernel<T, POLICY, GRAD, 128>, grid, size, 128, a)
+                          : launch(st, sweep_kernel<T, POLICY, GRAD, 256>, grid, size, 256, a);
 }
 
 // dlogits may be logits itself or must not touch it.
@@ -624,14 +641,11 @@ int pk_token_logprob_bwd(void* stream, int dtype, const void* logits, int64_t ld
     // few rows: several blocks to a row, down to two vectors per thread (80 rows of 32000 bf16: 9.7 -> 7.0 us)
     const int64_t most = std::max<int64_t>(1, V * static_cast<int64_t>(dtype_size(dtype)) / (threads * 32));
     const dim3 grid(row_blocks(R), static_cast<unsigned>(std::min<int64_t>(most, std::max<int64_t>(1, sm_count() * 4 / R))));
-    if (dtype == PK_F32)
-        token_logprob_bwd_kernel<float><<<grid, threads, 0, as_stream(stream)>>>(
-            static_cast<const float*>(logits), ld, targets, lse, dlogp, static_cast<float*>(dlogits), ldd, R, V, status);
-    else
-        token_logprob_bwd_kernel<bf16><<<grid, threads, 0, as_stream(stream)>>>(
-            static_cast<const bf16*>(logits), ld, targets, lse, dlogp, static_cast<bf16*>(dlogits), ldd, R, V, status);
-    PK_LAUNCH_CHECK();
-    return PK_OK;
+    cudaStream_t st = as_stream(stream);
+    return dtype == PK_F32 ? launch(st, token_logprob_bwd_kernel<float>, grid, 1, threads, static_cast<const float*>(logits), ld, targets,
+                                    lse, dlogp, static_cast<float*>(dlogits), ldd, R, V, status)
+                           : launch(st, token_logprob_bwd_kernel<bf16>, grid, 1, threads, static_cast<const bf16*>(logits), ld, targets,
+                                    lse, dlogp, static_cast<bf16*>(dlogits), ldd, R, V, status);
 }
 
 int pk_preference_loss(void* stream, const float* logp, const float* ref_logp, const float* weight,
@@ -641,10 +655,8 @@ int pk_preference_loss(void* stream, const float* logp, const float* ref_logp, c
     PK_REQUIRE(label_smoothing >= 0.0f && label_smoothing <= 1.0f, "label_smoothing must be in [0, 1]");
     if (n_pairs == 0) return PK_OK;
     PK_REQUIRE(seq && loss && (R == 0 || logp), "null pointer");
-    preference_loss_kernel<<<static_cast<unsigned>(n_pairs), PAIR_THREADS, 0, as_stream(stream)>>>(
-        logp, ref_logp, weight, seq, R, beta, label_smoothing, grad_scale, loss, margin, dlogp, status);
-    PK_LAUNCH_CHECK();
-    return PK_OK;
+    return launch(as_stream(stream), preference_loss_kernel, dim3(static_cast<unsigned>(n_pairs)), 1, PAIR_THREADS, logp, ref_logp, weight, seq,
+                  R, beta, label_smoothing, grad_scale, loss, margin, dlogp, status);
 }
 
 int pk_policy_loss(void* stream, int dtype, const void* logits, int64_t ld, const int32_t* targets,
