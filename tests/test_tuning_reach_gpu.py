@@ -164,6 +164,60 @@ def test_two_streams_at_once(pk):  # noqa: F811
             assert all(torch.equal(a[k], b[k]) for k in a)
 
 
+@pytest.mark.parametrize("R, V", [(40, 32000), (2000, 515), (3000, 8192)])
+def test_calls_wait_for_what_runs_before_them(pk, R, V):  # noqa: F811
+    """Kernels that start early still see what their predecessors write and leave alone what those read: other kernels, copies,
+    each other, and a join of two streams, on a stream and in a graph."""
+    base, t = ops.make_logits(R, V, V, 0, torch.bfloat16)
+    ti, adv, old = t.to(torch.int32), torch.randn(R, device="cuda", generator=gen(3)), torch.full((R,), -9.0, device="cuda")
+    seq = torch.tensor([0, R // 4, R // 2, R // 2 + 3, R], dtype=torch.int32, device="cuda")
+    x, x2 = torch.zeros_like(base), torch.zeros_like(base)
+    o = {k: torch.zeros(n, device="cuda") for k, n in (("logp", R), ("lse", R), ("loss", 2), ("dlogp", R), ("rl", R), ("dw", 64))}
+    heads, gain = torch.randn(R, 64, device="cuda", generator=gen(4)), torch.ones(64, device="cuda")
+    s_heads = scratch(pk.pk_qk_norm_rope_bwd_scratch_bytes(R, 1, 0, 64))
+    dheads = torch.zeros_like(heads)
+    side = torch.cuda.Stream()
+
+    def work(scale, wait=lambda: None):
+        here = torch.cuda.current_stream()
+        torch.mul(base, scale, out=x)                      # a kernel right before
+        wait()
+        pkt.check(pk.pk_token_logprob(stream(), 1, ptr(x), V, ptr(ti), None, ptr(o["logp"]), ptr(o["lse"]), R, V, None))
+        wait()
+        pkt.check(pk.pk_preference_loss(stream(), ptr(o["logp"]), None, None, ptr(seq), 2, R, 0.1, 0.0, 1.0, ptr(o["loss"]), None, ptr(o["dlogp"]), None))
+        wait()
+        pkt.check(pk.pk_token_logprob_bwd(stream(), 1, ptr(x), V, ptr(ti), ptr(o["lse"]), ptr(o["dlogp"]), ptr(x), V, R, V, None))
+        side.wait_stream(here)
+        with torch.cuda.stream(side):
+            x2.copy_(x)                                    # another stream between
+        here.wait_stream(side)
+        wait()
+        pkt.check(pk.pk_policy_loss(stream(), 1, ptr(x2), V, ptr(ti), ptr(old), None, ptr(adv), None, 0.2, 0.2, 0.0, 1.0, ptr(o["rl"]), None, None,
+                                    ptr(x2), V, R, V, None))
+        wait()
+        o["dw"].zero_()
+        pkt.check(pk.pk_qk_norm_rope_bwd(stream(), 0, ptr(heads), 64, None, 0, ptr(heads), 64, None, 0, ptr(gain), None, ptr(dheads), 64, None, 0,
+                                         ptr(o["dw"]), None, ptr(s_heads), R, 1, 0, 64, 0, 0, 1e-5, None, None, 0))
+        wait()
+        return [v.clone() for v in (*o.values(), x, x2, dheads)]
+
+    want = {k: work(k, torch.cuda.synchronize) for k in (1.0, 0.5, 2.0)}
+    for i in range(30):
+        k = (1.0, 0.5, 2.0)[i % 3]
+        got = work(k)
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want[k]))
+    graph, main = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    with torch.cuda.graph(graph, stream=main):
+        got = work(0.5)
+    for _ in range(5):
+        for v in got:
+            v.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want[0.5]))
+
+
 FIRST = r'''
 import torch
 from tests import pkt
