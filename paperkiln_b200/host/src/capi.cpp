@@ -44,6 +44,8 @@ struct Model {
     std::unique_ptr<dp::GradientExchange> exchange;   // data-parallel gradient exchange (mt_dp_*)
     float lr = 1e-3f, b1 = 0.9f, b2 = 0.999f, eps = 1e-8f, wd = 0.01f;
     int state_bits = 32;
+    struct Rate { float lr_mult, weight_decay; };
+    std::map<size_t, Rate> rates;   // by optimizer index; kept until there is an optimizer
     int64_t live_after_fwd = 0;
     size_t loss_chunk = 16384;
     bool accumulate = false;   // mt_model_step keeps the gradients it finds
@@ -685,6 +687,7 @@ static nn::AdamW& optimizer(Model* m) {
     if (!m->opt) {
         m->opt = std::make_unique<nn::AdamW>(m->params, m->lr, m->b1, m->b2, m->eps, m->wd);
         m->opt->set_state_bits(m->state_bits);
+        for (const auto& [i, r] : m->rates) m->opt->set_rates(i, r.lr_mult, r.weight_decay);
     }
     return *m->opt;
 }
@@ -708,7 +711,9 @@ int mt_model_set_adamw_state_bits(void* h, int bits) {
 int mt_model_set_param_rates(void* h, int64_t i, float lr_mult, float weight_decay) {
     return guard([&] {
         Model* m = M(h);
-        optimizer(m).set_rates(optimizer_index(m, i), lr_mult, weight_decay);
+        const size_t k = optimizer_index(m, i);
+        m->rates[k] = {lr_mult, weight_decay};
+        if (m->opt) m->opt->set_rates(k, lr_mult, weight_decay);
     });
 }
 int mt_model_optimizer_step(void* h) {

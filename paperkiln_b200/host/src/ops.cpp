@@ -1120,6 +1120,7 @@ Var attention_qk_norm(const Var& q, const Var& k, const Var& v, const Var& wq, c
     if (wq->data.rows() != 1 || wq->data.cols() != dk || wk->data.rows() != 1 || wk->data.cols() != dk)
         throw std::runtime_error("attention_qk_norm: gains must be [1, head_dim]");
     if (dk % 2 != 0 || rot_q > Hq || rot_k > Hkv) throw std::runtime_error("attention_qk_norm: bad rotation");
+    if (wq == wk) throw std::runtime_error("attention_qk_norm: queries and keys need a gain each");
     if (pos.size() != T) throw std::runtime_error("attention_qk_norm: one position per row");
     const size_t sl = seq_len == 0 ? T : seq_len;
     if (sl == 0 || T % sl != 0) throw std::runtime_error("attention_qk_norm: rows not a multiple of seq_len");

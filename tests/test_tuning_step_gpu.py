@@ -274,6 +274,18 @@ def test_rates_of_single_parameters(mt, bits):
     assert np.abs(diff - 1e-2 * 0.1).max() <= 4 * 2.0 ** -24
 
 
+def test_optimizer_settings_in_any_order(mt):
+    """Rates before the hyper-parameters, bits between them: the same run."""
+    a = train(mt, 2, 8, rates={"norm.weight": (0.5, 0.0)})
+    b = mt.Model(**SPEC)
+    b.set_param_rates("norm.weight", 0.5, 0.0)
+    b.set_adamw_state_bits(8)
+    b.set_adamw(lr=1e-2, weight_decay=0.1)
+    train(mt, 2, model=b)
+    for n in a.names:
+        assert np.array_equal(a.get_param(n), b.get_param(n)), n
+
+
 @pytest.mark.parametrize("dtype", ["fp32", "bf16"])
 def test_eight_bit_moments_follow_the_gradients(mt, dtype):
     mt.init(0, mt.BF16 if dtype == "bf16" else mt.FP32)
