@@ -311,19 +311,20 @@ __device__ __forceinline__ uint4 pack(const float (&f)[8]) {
 // Nothing orders the rows: the chain from a row's last byte over its reductions to its scalars is hidden by
 // what else is resident.
 //
-// Bound by memory and its latency. Policy loss with its gradient, bf16: 8192 x 32000 184 us, 5.7 TB/s (second
-// reading forwards 192; past L1 242), 60000 x 4000 160 us, 6.0 TB/s. A row that stays in the registers or the
-// shared memory of its CTAs while the next one is on its way with cp.async took 207 and 385: its warps wait
-// for one another between the rows. Without a gradient: 8192 x 50257 150 us, 5.5 TB/s.
+// Bound by memory and its latency. Policy loss with its gradient, bf16: 8192 x 32000 189 us, 5.5 TB/s (second
+// reading forwards 195), 60000 x 4000 168 us, 5.7 TB/s, 8192 x 151936 928 us, 5.4 TB/s. A row that stays in the
+// registers or the shared memory of its CTAs while the next one is on its way with cp.async took 207 at the first size
+// and 385 at the second: its warps wait for one another between the rows. Holding a part of the stretch in
+// shared memory for the second reading costs L1 as much as it saves (190; five CTAs per SM). Without a gradient:
+// 8192 x 50257 150 us, 5.5 TB/s.
 constexpr int CLUSTER_MOST = 8, SWEEP_K = 4;
 template <bool GRAD, int THREADS> struct Sweep {
     static constexpr int CTA = THREADS < 128 ? 128 : THREADS;  // threads of a CTA
     static constexpr int PER_SM = GRAD ? (CTA == 128 ? 10 : 6) : 2048 / CTA;
 };
 
-// The second reading is the last, and nobody reads the gradient before the kernel's end: both are marked to
-// leave L2 first, so that they do not push out stretches that have yet to be read again (8192 x 32000 bf16 219 -> 192 us
-// before the second reading went backwards).
+// The second reading is the last, and nobody reads the gradient before the kernel's end: both are marked to leave L2
+// first, so that they do not push out stretches that have yet to be read again (8192 x 32000 bf16 209 -> 189 us).
 __device__ __forceinline__ uint4 load_last(const void* p) { return __ldcs(static_cast<const uint4*>(p)); }
 
 template <typename T, bool POLICY, bool GRAD, int THREADS>
@@ -616,9 +617,9 @@ int launch_rows(cudaStream_t st, const RowArgs& a) {
     constexpr int N = Vec<T>::N;
     const int64_t vectors = (a.V + N - 1) / N;
     const int sms = sm_count();
-    // Threads per row, us with a gradient in bf16 for 32 / 128 / 256: 32000 x 6000 139 / 164 / 201, 32000 x 8000
-    // 188 / 184 / 217, 16000 x 16000 - / 174 / 180, 12000 x 24000 - / 207 / 197. Few rows take more: 1000 x 3000
-    // 12.3 / 10.2 / 14.3, 400 x 6000 16.4 / 12.3 / 10.2.
+    // Threads per row, us with a gradient in bf16 for 32 / 128 / 256: 32000 x 6000 145 / 178 / 221, 32000 x 8000
+    // 203 / 201 / 240, 16000 x 16000 - / 182 / 195, 12000 x 24000 - / 218 / 207. Few rows take more: 400 x 6000
+    // 16 / 12 / 12.
     int threads = vectors <= 896 ? 32 : (vectors <= 2048 ? 128 : 256);
     if (threads == 32 && vectors >= 256 && a.R <= sms * 8) threads = 128;
     if (threads == 128 && vectors >= 512 && a.R <= sms * 4) threads = 256;
@@ -626,7 +627,7 @@ int launch_rows(cudaStream_t st, const RowArgs& a) {
     if (threads == 32) return launch(st, sweep_kernel<T, POLICY, GRAD, 32>, dim3(static_cast<unsigned>((a.R + 3) / 4)), 1, 128, a);
     int size = 1;
     // With a gradient a CTA's stretch is at most 100 KB, so that the stretches of all resident CTAs stay in L2:
-    // 2048 x 151936 bf16 295 us with one CTA per row, 262 with two, 240 with four, 276 with eight.
+    // 2048 x 151936 bf16 295 us with one CTA per row, 266 with two, 246 with four, 292 with eight.
     if (GRAD)
         while (size < CLUSTER_MOST && vectors > static_cast<int64_t>(6400) * size) size *= 2;
     // few rows: as many CTAs as are resident, down to two vectors per thread (100 x 151936 bf16 without a gradient:
