@@ -363,7 +363,7 @@ int pk_fill(void* stream, int dtype, void* dst, float value, int64_t n);
  * +inf, or nothing but -inf, gives NaN, as its softmax does. A row that counts and whose target
  * is out of range reports it and gives 0 and a zero gradient. Logits may start anywhere and have any
  * row stride >= V; every gradient is written to dlogits [R, V] (row stride ldd), which may be logits
- * itself (then ldd == ld); any other overlap is refused.
+ * itself (then ldd == ld); any other overlap is refused, and so are more than 2^28 - 1 rows.
  *
  * logp[i] = logits[i, t_i] - lse[i], lse[i] = log(sum_j exp(logits[i, j])), fp32. weight may be NULL
  * (every row counts). The backward writes dlogits[i, j] = dlogp[i] * ([j == t_i] - exp(logits[i, j] - lse[i]));

@@ -306,10 +306,10 @@ __device__ __forceinline__ uint4 pack(const float (&f)[8]) {
 // A row belongs to a warp (THREADS = 32, four rows to a CTA), a CTA, or a cluster of 2 to 8 CTAs with a
 // stretch of it each. A thread holds K vectors in flight and a running sum of exponentials against its
 // running maximum. (A reference that follows the maximum only when that has moved by 8 saves no time, and
-// costs the large terms' exponents a rounding at 2^-21.) With a gradient the stretch is read once more, backwards: what was
-// read last is still in L1, and the stretches of all resident CTAs are in L2, so DRAM sees the logits once.
-// Nothing orders the rows: the chain from a row's last byte over its reductions to its scalars is hidden by
-// what else is resident.
+// costs the large terms' exponents a rounding at 2^-21.) With a gradient the stretch is read once more,
+// backwards: what was read last is still in L1, and the stretches of all resident CTAs are in L2, so DRAM sees the
+// logits once. Nothing orders the rows: the chain from a row's last byte over its reductions to its scalars is
+// hidden by what else is resident.
 //
 // Bound by memory and its latency. Policy loss with its gradient, bf16: 8192 x 32000 189 us, 5.5 TB/s (second
 // reading forwards 195), 60000 x 4000 168 us, 5.7 TB/s, 8192 x 151936 928 us, 5.4 TB/s. A row that stays in the
@@ -318,6 +318,7 @@ __device__ __forceinline__ uint4 pack(const float (&f)[8]) {
 // shared memory for the second reading costs L1 as much as it saves (190; five CTAs per SM). Without a gradient:
 // 8192 x 50257 150 us, 5.5 TB/s.
 constexpr int CLUSTER_MOST = 8, SWEEP_K = 4;
+constexpr int64_t ROWS_MOST = 0x7fffffff / CLUSTER_MOST;  // of a call with one grid for all rows
 template <bool GRAD, int THREADS> struct Sweep {
     static constexpr int CTA = THREADS < 128 ? 128 : THREADS;  // threads of a CTA
     static constexpr int PER_SM = GRAD ? (CTA == 128 ? 10 : 6) : 2048 / CTA;
@@ -623,7 +624,6 @@ int launch_rows(cudaStream_t st, const RowArgs& a) {
     int threads = vectors <= 896 ? 32 : (vectors <= 2048 ? 128 : 256);
     if (threads == 32 && vectors >= 256 && a.R <= sms * 8) threads = 128;
     if (threads == 128 && vectors >= 512 && a.R <= sms * 4) threads = 256;
-    PK_REQUIRE(a.R <= 0x7fffffff / CLUSTER_MOST, "too many rows");
     if (threads == 32) return launch(st, sweep_kernel<T, POLICY, GRAD, 32>, dim3(static_cast<unsigned>((a.R + 3) / 4)), 1, 128, a);
     int size = 1;
     // With a gradient a CTA's stretch is at most 100 KB, so that the stretches of all resident CTAs stay in L2:
@@ -658,6 +658,7 @@ int pk_token_logprob(void* stream, int dtype, const void* logits, int64_t ld, co
                      const float* weight, float* logp, float* lse, int64_t R, int64_t V, int32_t* status) {
     PK_REQUIRE(valid_dtype(dtype), "bad dtype");
     PK_REQUIRE(R >= 0 && V > 0 && ld >= V, "bad shape");
+    PK_REQUIRE(R <= ROWS_MOST, "too many rows");
     if (R == 0) return PK_OK;
     PK_REQUIRE(logits && targets && logp && lse, "null pointer");
     RowArgs a{};
@@ -702,6 +703,7 @@ int pk_policy_loss(void* stream, int dtype, const void* logits, int64_t ld, cons
                    float* kl, void* dlogits, int64_t ldd, int64_t R, int64_t V, int32_t* status) {
     PK_REQUIRE(valid_dtype(dtype), "bad dtype");
     PK_REQUIRE(R >= 0 && V > 0 && ld >= V && (dlogits == nullptr || ldd >= V), "bad shape");
+    PK_REQUIRE(R <= ROWS_MOST, "too many rows");
     PK_REQUIRE(clip_lo >= 0.0f && clip_lo <= 1.0f && clip_hi >= 0.0f, "clip bounds must not be negative, the lower at most 1");
     if (R == 0) return PK_OK;
     PK_REQUIRE(logits && targets && advantage && row_loss, "null pointer");

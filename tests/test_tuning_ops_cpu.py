@@ -41,6 +41,12 @@ def test_token_logprob_refusals(pk):
     assert b(None, 0, None, 8, None, None, None, None, 8, 0, 8, None) == 0
 
 
+def test_more_rows_than_a_grid_holds(pk):
+    R = 1 << 28
+    refused(pk, pk.pk_token_logprob(None, 0, P, 8, P, None, P, P, R, 8, None), b"too many rows")
+    refused(pk, pk.pk_policy_loss(None, 1, P, 8, P, None, None, P, None, 0.2, 0.2, 0.0, 1.0, P, None, None, None, 8, R, 8, None), b"too many rows")
+
+
 def test_preference_refusals(pk):
     f = pk.pk_preference_loss
     refused(pk, f(None, P, P, None, P, -1, 4, 0.1, 0.0, 1.0, P, None, None, None), b"shape")

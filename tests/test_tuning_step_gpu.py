@@ -158,6 +158,53 @@ def test_policy_gradient_of_a_fresh_policy_is_the_cross_entropy_gradient(mt, fam
     assert half["loss"] == out["loss"]
 
 
+def test_flex_models_and_heads_apart(mt):
+    """The flex family's untied head: policy and preference gradients against each other and the cross entropy's."""
+    m = mt.Model(family="flex", vocab=131, d=64, layers=2, heads=4, dff=96, nctx=64, norm="rmsnorm", act="swiglu", pos="sinusoidal", seed=3)
+    ids, targets = tokens(32, vocab=131)
+    m.step(ids, targets, 16)
+    want = m.grads()
+    m.policy_step(ids, targets, np.ones(32), 16, weight=np.full(32, 1 / 32))
+    close_grads(m.grads(), want)
+    out = m.preference_step(ids, targets, [0, 16, 32], 16, beta=0.2)
+    got = m.grads()
+    lp = m.token_logprob(ids, targets, 16).astype(np.float64)
+    z = 0.2 * (lp[:16].sum() - lp[16:].sum())
+    assert abs(out["margin"][0] - z) <= 1e-5 * max(1, abs(z))
+    dlogp = -0.2 / (1 + np.exp(z)) * np.repeat([1.0, -1.0], 16)
+    m.policy_step(ids, targets, -dlogp, 16)
+    close_grads(got, m.grads())
+
+
+@pytest.mark.parametrize("chunk", [0, 7])
+def test_micro_batches_add_up(mt, chunk):
+    """Two accumulated halves give the gradient of the whole batch, for both losses; a step without backward leaves it alone."""
+    ids, targets = tokens(64)
+    adv = np.random.RandomState(4).randn(64)
+    old = -5 + 0.1 * np.random.RandomState(5).randn(64)
+    seq = np.arange(0, 65, 16, dtype=np.int32)
+    whole = mt.Model(**SPEC, ckpt=1)
+    halves = mt.Model(**SPEC, ckpt=1)
+    halves.set_loss_chunk(chunk)
+    for kind in ("policy", "preference"):
+        if kind == "policy":
+            run = lambda m, a, b, scale: m.policy_step(ids[a:b], targets[a:b], adv[a:b], 16, old_logp=old[a:b], loss_scale=scale)  # noqa: E731
+            run(whole, 0, 64, 1.0)
+        else:
+            run = lambda m, a, b, scale: m.preference_step(ids[a:b], targets[a:b], seq[:(b - a) // 16 + 1], 16, loss_scale=scale)  # noqa: E731
+            run(whole, 0, 64, 1.0)
+        want = whole.grads()
+        halves.zero_grad()
+        halves.set_accumulate(True)
+        scale = 1.0 if kind == "policy" else 0.5   # a sum over rows; a mean over pairs
+        run(halves, 0, 32, scale)
+        halves.policy_step(ids, targets, adv, 16, backward=False)
+        halves.token_logprob(ids, targets, 16)
+        run(halves, 32, 64, scale)
+        halves.set_accumulate(False)
+        close_grads(halves.grads(), want)
+
+
 def test_policy_step_values_and_rows_that_do_not_count(mt):
     m = mt.Model(**SPEC, ckpt=1)
     m.set_loss_chunk(17)
