@@ -140,8 +140,8 @@ __device__ __forceinline__ void adamw_element(float& p, float g, float& m, float
     p = __fmaf_rn(-s.lr, __fmaf_rn(s.wd, p, upd), p);
 }
 
-// sqrt(x) within half a unit of the last place and a hair: an approximate reciprocal root and one
-// Newton step on its product with x. (The correctly rounded form takes 13 % of the kernel's time; the
+// sqrt(x) within half a unit of the last place and a hair: with q near 1 / sqrt(x) and s = x q, one step of Newton's
+// iteration for s^2 = x, s + (x - s^2) / (2 s), where 1 / (2 s) is taken as q / 2. (The correctly rounded form takes 13 % of the kernel's time; the
 // approximate one alone, two units off, moves one stored code in 10^5 to its neighbour.) Below the
 // smallest normal number the approximation serves.
 __device__ __forceinline__ float root(float x) {

@@ -66,6 +66,7 @@ struct Base {
         return tc::f2_pack(ex2(lo), ex2(hi));
     }
 };
+
 // A row of V values that may start anywhere: `head` values up to the first 16-byte boundary, nv
 // vectors, and a tail.
 template <typename T> struct RowSplit {
@@ -144,7 +145,7 @@ token_logprob_bwd_kernel(const T* logits, int64_t ld, const int32_t* __restrict_
 // k times the upper bits of log(2) is exact, and what the sums round off is carried along. A logarithm of fp32
 // taken whole rounds at its own size, and its sum with m once more; a KL term of two close policies feels both.
 constexpr float LN2_HI = 11355.0f / 16384, LN2_LO = 9.2981341195e-5f;
-__device__ __forceinline__ float sum2(float a, float b, float& left) {  // a + b, and what its rounding left out
+__device__ __forceinline__ float sum2(float a, float b, float& left) {  // a + b, and what its rounding left out (Knuth's two-sum)
     const float c = __fadd_rn(a, b), t = __fsub_rn(c, a);
     left += __fadd_rn(__fsub_rn(a, __fsub_rn(c, t)), __fsub_rn(b, t));
     return c;
