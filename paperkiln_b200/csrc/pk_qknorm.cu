@@ -21,7 +21,10 @@
 namespace pk {
 namespace {
 
-constexpr int THREADS = 256, WARPS = THREADS / 32;
+constexpr int THREADS = 256, WARPS = THREADS / 32;  // of the backward
+// Small CTAs in the forward, nine to an SM at 56 registers (65536 x 40 heads of 64: 120 us; four of 256 at 64
+// registers 130, ten at 48 120, and 118 against 114 at head_dim 128).
+constexpr int FWD_THREADS = 128, FWD_WARPS = FWD_THREADS / 32;
 constexpr int U = 4;  // heads per team in flight, at most
 
 // One kind of heads (queries or keys) and how its tasks are cut.
@@ -33,7 +36,7 @@ struct Kind {
     const float* w;
     int heads, rot;
     int step;             // heads side by side in a warp: a power of two, at most the warp's teams
-    int u;                // heads per team and task: U, or what divides the heads evenly
+    int u;                // heads per team and task: at most U (7 in the forward), chosen so that rounds are full
     int rounds;           // tasks per group of tokens (teams / step tokens)
     int64_t groups;
     int blocks;           // backward: blocks that work on this kind
@@ -158,11 +161,15 @@ __device__ __forceinline__ const float* table_row(const QkArgs& a, int64_t p) {
 // does), they are left out.
 enum Form { ANY = 0, FULL_TURN = 1, FULL_PLAIN = 2 };
 template <Form F, int UU> struct Shape {};
-template <typename T, int N, int LANES, int PIECES, typename Run>
+template <typename T, int N, int LANES, int PIECES, bool BACK, typename Run>
 __device__ __forceinline__ void with_shape(const QkArgs& a, const Kind& k, int first, bool tokens, Run run) {
     const int last = first + k.step * k.u;
     const bool full = last <= k.heads && PIECES * LANES * N == a.dk && tokens;
     const bool turn = full && last <= k.rot, plain = full && first >= k.rot;
+    if constexpr (!BACK) {
+        if (k.u == 7) return turn ? run(Shape<FULL_TURN, 7>()) : run(Shape<ANY, 7>());
+        if (turn && k.u == 3) return run(Shape<FULL_TURN, 3>());
+    }
     if (turn && k.u == 4) run(Shape<FULL_TURN, 4>());
     else if (turn && k.u == 2) run(Shape<FULL_TURN, 2>());
     else if (turn) run(Shape<FULL_TURN, 1>());
@@ -244,18 +251,18 @@ __device__ __forceinline__ void forward_task(const QkArgs& a, const Kind& k, con
 }
 
 template <typename T, int N, int LANES, int PIECES>
-__global__ void __launch_bounds__(THREADS, PIECES == 1 ? 4 : 1)
+__global__ void __launch_bounds__(FWD_THREADS, PIECES == 1 ? 9 : 1)
 qk_norm_rope_fwd_kernel(QkArgs a) {
     constexpr int TEAMS = 32 / LANES;
     const Place<T, N, LANES, PIECES> at;
     const bool keys = static_cast<int>(blockIdx.y) >= a.kind[0].rounds;
     const Kind& k = a.kind[keys];
     const int first = (static_cast<int>(blockIdx.y) - (keys ? a.kind[0].rounds : 0)) * k.step * k.u;
-    const int64_t group = static_cast<int64_t>(blockIdx.x) * WARPS + (threadIdx.x >> 5);
+    const int64_t group = static_cast<int64_t>(blockIdx.x) * FWD_WARPS + (threadIdx.x >> 5);
     if (group >= k.groups) return;
     const int per = TEAMS / k.step;
     const int64_t t = group * per + at.team / k.step;
-    with_shape<T, N, LANES, PIECES>(a, k, first, (group + 1) * per <= a.T, [&](auto shape) { forward_task(a, k, at, t, first, shape); });
+    with_shape<T, N, LANES, PIECES, false>(a, k, first, (group + 1) * per <= a.T, [&](auto shape) { forward_task(a, k, at, t, first, shape); });
 }
 
 // One task of the backward; adds the thread's share of dw.
@@ -355,7 +362,7 @@ qk_norm_rope_bwd_kernel(QkArgs a) {
         T* y = static_cast<T*>(k.y) + t * k.ldy + c0;
         const bool turns = a.pos != nullptr;
         int64_t p = turns && t < a.T ? a.pos[t] : 0;
-        with_shape<T, N, LANES, PIECES>(a, k, first, a.T % per == 0, [&](auto shape) {
+        with_shape<T, N, LANES, PIECES, true>(a, k, first, a.T % per == 0, [&](auto shape) {
             for (; t <= end; t += hop, x += hop * k.ldx, g += hop * k.ldg, y += hop * k.ldy) {
                 const int64_t ahead = turns && t + hop < a.T ? a.pos[t + hop] : 0;
                 backward_task(a, k, at, x, g, y, first, t < a.T, p, w, dw, shape);
@@ -417,12 +424,21 @@ int blocks_of(int heads, int others, int rounds) {
     const int share = static_cast<int>(std::max<int64_t>(1, wave * heads / (static_cast<int64_t>(heads) + others)));
     return std::max(share, (rounds + WARPS - 1) / WARPS);
 }
-void cut(QkArgs& a, int teams) {
+void cut(QkArgs& a, int teams, bool back) {
     for (Kind& k : a.kind) {
         k.step = 1;
         while (k.step < teams && k.step < k.heads) k.step *= 2;
         // a round of U heads per team; fewer where that leaves no round half empty
         k.u = k.heads % (k.step * U) == 0 || k.heads > k.step * U ? U : (k.heads % (k.step * 2) == 0 ? 2 : (k.heads <= k.step ? 1 : U));
+        // head counts that this leaves ragged: fewer side by side, in full rounds of 4, 7 or 3 (forward of 65536 x 14 / 2 heads of
+        // 64: XX us)
+        for (int s = k.step; !back && s > 0 && k.heads % (k.step * k.u) != 0; s /= 2)
+            for (int u : {4, 7, 3})
+                if (k.heads % (s * u) == 0) {
+                    k.step = s;
+                    k.u = u;
+                    break;
+                }
         k.rounds = (k.heads + k.step * k.u - 1) / (k.step * k.u);
         k.groups = (a.T + teams / k.step - 1) / (teams / k.step);
     }
@@ -430,7 +446,7 @@ void cut(QkArgs& a, int teams) {
 
 template <typename T, int N, int LANES, int PIECES, bool BACK>
 int launch(cudaStream_t st, QkArgs a, int (&blocks)[2]) {
-    cut(a, 32 / LANES);
+    cut(a, 32 / LANES, BACK);
     if constexpr (BACK) {
         for (int r = 0; r < 2; ++r) {
             Kind& k = a.kind[r];
@@ -441,10 +457,10 @@ int launch(cudaStream_t st, QkArgs a, int (&blocks)[2]) {
         }
         qk_norm_rope_bwd_kernel<T, N, LANES, PIECES><<<static_cast<unsigned>(blocks[0] + blocks[1]), THREADS, 0, st>>>(a);
     } else {
-        const int64_t gx = (std::max(a.kind[0].heads ? a.kind[0].groups : 0, a.kind[1].heads ? a.kind[1].groups : 0) + WARPS - 1) / WARPS;
+        const int64_t gx = (std::max(a.kind[0].heads ? a.kind[0].groups : 0, a.kind[1].heads ? a.kind[1].groups : 0) + FWD_WARPS - 1) / FWD_WARPS;
         const int gy = a.kind[0].rounds + a.kind[1].rounds;
         PK_REQUIRE(gx <= 0x7fffffff && gy <= 65535, "too many rows or heads");
-        qk_norm_rope_fwd_kernel<T, N, LANES, PIECES><<<dim3(static_cast<unsigned>(gx), gy), THREADS, 0, st>>>(a);
+        qk_norm_rope_fwd_kernel<T, N, LANES, PIECES><<<dim3(static_cast<unsigned>(gx), gy), FWD_THREADS, 0, st>>>(a);
     }
     PK_LAUNCH_CHECK();
     return PK_OK;
