@@ -159,16 +159,18 @@ __device__ __forceinline__ const float* table_row(const QkArgs& a, int64_t p) {
 // What a warp's task is like as a whole. The bounds, and whether a head turns, are a third of the
 // instructions of a task; where every head of the round exists, fills its lanes and turns (or none
 // does), they are left out.
-enum Form { ANY = 0, FULL_TURN = 1, FULL_PLAIN = 2 };
+enum Form { ANY = 0, FULL_TURN = 1, FULL_PLAIN = 2, PART_TURN = 3 };  // PART: lanes past dk are idle
 template <Form F, int UU> struct Shape {};
 template <typename T, int N, int LANES, int PIECES, bool BACK, typename Run>
 __device__ __forceinline__ void with_shape(const QkArgs& a, const Kind& k, int first, bool tokens, Run run) {
     const int last = first + k.step * k.u;
-    const bool full = last <= k.heads && PIECES * LANES * N == a.dk && tokens;
+    const bool heads = last <= k.heads && tokens, full = heads && PIECES * LANES * N == a.dk;
     const bool turn = full && last <= k.rot, plain = full && first >= k.rot;
     if constexpr (!BACK) {
-        if (k.u == 7) return turn ? run(Shape<FULL_TURN, 7>()) : run(Shape<ANY, 7>());
+        const bool part = heads && !full && last <= k.rot;
+        if (k.u == 7) return turn ? run(Shape<FULL_TURN, 7>()) : (part ? run(Shape<PART_TURN, 7>()) : run(Shape<ANY, 7>()));
         if (turn && k.u == 3) return run(Shape<FULL_TURN, 3>());
+        if (part) return k.u == 1 ? run(Shape<PART_TURN, 1>()) : (k.u == 2 ? run(Shape<PART_TURN, 2>()) : (k.u == 3 ? run(Shape<PART_TURN, 3>()) : run(Shape<PART_TURN, 4>())));
     }
     if (turn && k.u == 4) run(Shape<FULL_TURN, 4>());
     else if (turn && k.u == 2) run(Shape<FULL_TURN, 2>());
@@ -180,6 +182,7 @@ __device__ __forceinline__ void with_shape(const QkArgs& a, const Kind& k, int f
 template <typename T, int N, int LANES, int PIECES, Form F, int UU>
 __device__ __forceinline__ void forward_task(const QkArgs& a, const Kind& k, const Place<T, N, LANES, PIECES>& at, int64_t t, int first,
                                              Shape<F, UU>) {
+    constexpr bool FULL = F == FULL_TURN || F == FULL_PLAIN, TURNS = F == FULL_TURN || F == PART_TURN;
     const int h0 = first + at.team % k.step;
     const bool token = F != ANY || t < a.T;
     const int heads = min(k.heads, first + k.step * k.u);  // ANY: where the round ends
@@ -187,14 +190,14 @@ __device__ __forceinline__ void forward_task(const QkArgs& a, const Kind& k, con
     const T* x = static_cast<const T*>(k.x) + t * k.ldx + h0 * a.dk + at.tl * N;
     T* y = static_cast<T*>(k.y) + t * k.ldy + h0 * a.dk + at.tl * N;
     int64_t p = 0;
-    if (F == FULL_TURN || (F == ANY && a.pos && token)) p = a.pos[t];
+    if (TURNS || (F == ANY && a.pos && token)) p = a.pos[t];
     uint4 raw[UU][PIECES];
 #pragma unroll
     for (int u = 0; u < UU; ++u)
 #pragma unroll
         for (int j = 0; j < PIECES; ++j) {
-            if (F == ANY) raw[u][j] = make_uint4(0, 0, 0, 0);
-            if (F != ANY || (token && h0 + u * k.step < heads && at.col(j) < a.dk))
+            if (F == ANY || F == PART_TURN) raw[u][j] = make_uint4(0, 0, 0, 0);
+            if (FULL || (at.col(j) < a.dk && (F == PART_TURN || (token && h0 + u * k.step < heads))))
                 raw[u][j] = Piece<T, N>::load_raw(x + u * hop + j * (LANES * N));
         }
     // gain and angle of a pair in one: with c, s the angle's and w, w' the pair's gains,
@@ -202,7 +205,7 @@ __device__ __forceinline__ void forward_task(const QkArgs& a, const Kind& k, con
     Piece<T, N> w[PIECES], wc[PIECES], ws[PIECES];  // ws.even = w s, ws.odd = -w' s
 #pragma unroll
     for (int j = 0; j < PIECES; ++j) w[j].table(k.w, at.col(j), a.dk);
-    if (F == FULL_TURN || (F == ANY && a.pos)) {
+    if (TURNS || (F == ANY && a.pos)) {
         const float* row = table_row(a, p);
 #pragma unroll
         for (int j = 0; j < PIECES; ++j) {
@@ -222,7 +225,7 @@ __device__ __forceinline__ void forward_task(const QkArgs& a, const Kind& k, con
     for (int u = 0; u < UU; ++u) {
         const int h = h0 + u * k.step;
         if (F == ANY && first + u * k.step >= heads) break;  // the same for the whole warp
-        const bool turn = F == FULL_TURN || (F == ANY && h < k.rot);
+        const bool turn = TURNS || (F == ANY && h < k.rot);
         uint64_t sq = 0;
         Piece<T, N> v[PIECES];
 #pragma unroll
@@ -245,7 +248,7 @@ __device__ __forceinline__ void forward_task(const QkArgs& a, const Kind& k, con
                     o.odd[i] = f2_mul(inv, f2_mul(v[j].odd[i], w[j].odd[i]));
                 }
             }
-            if (F != ANY || (token && h < heads && at.col(j) < a.dk)) o.store(y + u * hop + j * (LANES * N));
+            if (FULL || (at.col(j) < a.dk && (F == PART_TURN || (token && h < heads)))) o.store(y + u * hop + j * (LANES * N));
         }
     }
 }
@@ -432,8 +435,8 @@ void cut(QkArgs& a, int teams, bool back) {
         k.u = k.heads % (k.step * U) == 0 || k.heads > k.step * U ? U : (k.heads % (k.step * 2) == 0 ? 2 : (k.heads <= k.step ? 1 : U));
         // head counts that this leaves ragged: fewer side by side, in full rounds of 4, 7 or 3 (forward of 65536 x 14 / 2 heads of
         // 64: XX us)
-        for (int s = k.step; !back && s > 0 && k.heads % (k.step * k.u) != 0; s /= 2)
-            for (int u : {4, 7, 3})
+        for (int s = k.step; s > 0 && k.heads % (k.step * k.u) != 0; s /= 2)
+            for (int u : {4, back ? 2 : 7, back ? 2 : 3})
                 if (k.heads % (s * u) == 0) {
                     k.step = s;
                     k.u = u;
