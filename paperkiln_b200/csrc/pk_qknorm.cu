@@ -8,7 +8,7 @@
 // nothing saved by the forward and reduces once.
 //
 // Bound by memory: 2 (forward) or 3 (backward) accesses per element. bf16: 65536 x 40 heads of 64 take
-// 129 us forward, 5.2 TB/s; 16381 x 32 heads of 128 take 76 us backward, 5.3 TB/s, the sum of dw included.
+// 120 us forward, 5.6 TB/s; 16381 x 32 heads of 128 take 76 us backward, 5.3 TB/s, the sum of dw included.
 // A team of LANES threads owns a head, 16 bytes per thread. A warp's task is a group of heads of one kind
 // and one token (of several tokens where a token has fewer heads than the warp has teams): U heads per
 // team, all loaded before the first is computed, with the rotation table's row and the gains in registers.
@@ -419,13 +419,26 @@ qk_gain_grad_kernel(const float* __restrict__ partial, int nq, int nk, int dk, f
     }
 }
 
-// Blocks of the backward: one resident wave at 128 registers, shared out by heads, at least a warp
-// for every round of a kind.
-int blocks_of(int heads, int others, int rounds) {
-    if (heads == 0) return 0;
-    const int64_t wave = static_cast<int64_t>(sm_count()) * 2;
-    const int share = static_cast<int>(std::max<int64_t>(1, wave * heads / (static_cast<int64_t>(heads) + others)));
-    return std::max(share, (rounds + WARPS - 1) / WARPS);
+// Blocks of the backward: one resident wave at 128 registers, shared out by the tasks of a kind and what a task
+// takes, at least a warp for every round. A task of u heads per team takes about as long as u + 4 heads: its loads'
+// latency is that of four. (By heads alone the warps of few key heads were the last: 65536 x 32 / 8 heads of 64
+// 205 -> 176 us, 16 / 1 of 128 266 -> 160, 14 / 2 of 64 126 -> 98; u + 2 182 / 176 / 102, u + 6 179 / 159 / 99.)
+constexpr int TASK = 4;
+int wave_blocks() { return sm_count() * 2; }
+void share_blocks(QkArgs& a) {
+    double cost[2];
+    for (int r = 0; r < 2; ++r) {
+        const Kind& k = a.kind[r];
+        cost[r] = k.heads == 0 ? 0.0 : static_cast<double>(k.rounds) * static_cast<double>(k.groups) * (k.u + TASK);
+    }
+    for (int r = 0; r < 2; ++r) {
+        Kind& k = a.kind[r];
+        if (k.heads == 0) continue;
+        const int least = (k.rounds + WARPS - 1) / WARPS;
+        k.blocks = std::max(least, static_cast<int>(wave_blocks() * (cost[r] / (cost[0] + cost[1]))));
+        // a few tokens need no full wave
+        k.blocks = static_cast<int>(std::min<int64_t>(k.blocks, (k.groups * k.rounds + WARPS - 1) / WARPS));
+    }
 }
 void cut(QkArgs& a, int teams, bool back) {
     for (Kind& k : a.kind) {
@@ -433,9 +446,9 @@ void cut(QkArgs& a, int teams, bool back) {
         while (k.step < teams && k.step < k.heads) k.step *= 2;
         // a round of U heads per team; fewer where that leaves no round half empty
         k.u = k.heads % (k.step * U) == 0 || k.heads > k.step * U ? U : (k.heads % (k.step * 2) == 0 ? 2 : (k.heads <= k.step ? 1 : U));
-        // head counts that this leaves ragged: fewer side by side, in full rounds of 4, 7 or 3 (forward of 65536 x 14 / 2 heads of
-        // 64: XX us)
-        for (int s = k.step; s > 0 && k.heads % (k.step * k.u) != 0; s /= 2)
+        // Head counts that this leaves ragged: fewer side by side, in full rounds of 4, 7 or 3 (forward of 65536 x 14 / 2
+        // heads of 64: 77 -> 61 us). A few tokens have time for the bounds, not for longer tasks (37: 2.5 us, else 3.2).
+        for (int s = a.T >= 1024 ? k.step : 0; s > 0 && k.heads % (k.step * k.u) != 0; s /= 2)
             for (int u : {4, back ? 2 : 7, back ? 2 : 3})
                 if (k.heads % (s * u) == 0) {
                     k.step = s;
@@ -451,13 +464,8 @@ template <typename T, int N, int LANES, int PIECES, bool BACK>
 int launch(cudaStream_t st, QkArgs a, int (&blocks)[2]) {
     cut(a, 32 / LANES, BACK);
     if constexpr (BACK) {
-        for (int r = 0; r < 2; ++r) {
-            Kind& k = a.kind[r];
-            k.blocks = blocks_of(k.heads, a.kind[1 - r].heads, k.rounds);
-            // a few tokens need no full wave
-            if (k.blocks > 0) k.blocks = static_cast<int>(std::min<int64_t>(k.blocks, (k.groups * k.rounds + WARPS - 1) / WARPS));
-            blocks[r] = k.blocks;
-        }
+        share_blocks(a);
+        for (int r = 0; r < 2; ++r) blocks[r] = a.kind[r].blocks;
         qk_norm_rope_bwd_kernel<T, N, LANES, PIECES><<<static_cast<unsigned>(blocks[0] + blocks[1]), THREADS, 0, st>>>(a);
     } else {
         const int64_t gx = (std::max(a.kind[0].heads ? a.kind[0].groups : 0, a.kind[1].heads ? a.kind[1].groups : 0) + FWD_WARPS - 1) / FWD_WARPS;
@@ -542,8 +550,8 @@ int pk_qk_norm_rope_fwd(void* stream, int dtype, const void* q, int64_t ldq, con
 size_t pk_qk_norm_rope_bwd_scratch_bytes(int64_t T, int Hq, int Hkv, int head_dim) {
     (void)T;
     if (Hq < 0 || Hkv < 0 || head_dim <= 0) return 0;
-    // the most blocks of any form: a head per round makes the most rounds
-    const size_t blocks = static_cast<size_t>(blocks_of(Hq, Hkv, Hq)) + static_cast<size_t>(blocks_of(Hkv, Hq, Hkv));
+    // a wave, and a warp for every round where that is more: a head per round makes the most rounds
+    const size_t blocks = static_cast<size_t>(wave_blocks()) + static_cast<size_t>(Hq + WARPS - 1) / WARPS + static_cast<size_t>(Hkv + WARPS - 1) / WARPS;
     return blocks * static_cast<size_t>(head_dim) * sizeof(float);
 }
 

@@ -31,6 +31,15 @@ def test_masked_words_in_wide_vocabularies(pk, dtype, V):  # noqa: F811
     ops.test_masked_words_and_odd_rows(pk, dtype, V)
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("shape", [(1025, 14, 2, 64), (1100, 14, 2, 96), (1031, 3, 6, 80), (1024, 12, 12, 64), (1500, 7, 1, 256), (1026, 24, 3, 34),
+                                   (1501, 16, 1, 128), (1200, 6, 5, 64), (1027, 40, 0, 64), (1027, 0, 7, 32), (2051, 28, 4, 8)])
+@pytest.mark.parametrize("layout, turn", [("packed", "all"), ("apart", "first"), ("apart", "none"), ("unaligned", "all")])
+def test_head_norms_of_many_tokens(pk, dtype, shape, layout, turn):  # noqa: F811
+    """Rounds of heads are cut another way from a thousand tokens on."""
+    ops.test_qk_norm_rope(pk, dtype, shape, layout, turn)
+
+
 def policy(pk, x, t, old, adv, w, dx, ld, ldd, R, V, loss, logp):  # noqa: F811
     pkt.check(pk.pk_policy_loss(stream(), dt(x), ptr(x), ld, ptr(t), ptr(old), None, ptr(adv), ptr(w), 0.2, 0.2, 0.0, 1.0, ptr(loss),
                                 ptr(logp), None, ptr(dx), ldd, R, V, None))
