@@ -416,7 +416,7 @@ int pk_adamw(void* stream, float* p, const float* g, float* m, float* v, int64_t
  * state_bits = 8:  m and v are E4M3 codes [n] with one power-of-two scale per 32 elements, its
  *   exponent byte (2^(byte - 127), the E8M0 form) in m_scale / v_scale [ceil(n / 32)]: m = code * 2^(byte - 127),
  *   and v holds sqrt(v) the same way. The update itself uses the fp32 moments before they are
- *   rounded. m is rounded to nearest; sqrt(v) is rounded up or down at random with the right mean,
+ *   rounded; every product and sum of the moments is rounded to fp32 on its own. m is rounded to nearest; sqrt(v) is rounded up or down at random with the right mean,
  *   because with b2 = 0.999 a step moves v by less than half a code and rounding to nearest would
  *   freeze it; and no sqrt(v) above zero becomes zero. The random bits are a function of `seed` (pass
  *   another one every step) and the element's number in the plan: the same call gives the same
