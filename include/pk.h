@@ -423,7 +423,8 @@ int pk_adamw(void* stream, float* p, const float* g, float* m, float* v, int64_t
  *   bits. All-zero buffers are the initial state. A moment that is not finite is stored as NaN and
  *   does not enter its block's scale.
  * The plan is the device-side table of the tensors, made once (pk_adamw_plan_create allocates device
- * memory; call both outside stream captures, with the GPU current that holds the tensors). Every
+ * memory and waits until the table is there, so that a step may follow on any stream; call both outside
+ * stream captures, with the GPU current that holds the tensors). Every
  * buffer must lie on that GPU; no written buffer may overlap another one. The step itself allocates
  * nothing and may be captured; two steps of one plan must not run at the same time. */
 typedef struct pk_adamw_tensor {

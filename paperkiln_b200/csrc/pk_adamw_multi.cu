@@ -495,6 +495,9 @@ int pk_adamw_plan_create(const pk_adamw_tensor* tensors_h, int n_tensors, int g_
             void* dev = nullptr;
             cudaError_t e = cudaMalloc(&dev, bytes);
             if (e == cudaSuccess) e = cudaMemcpy(dev, chunks.data(), bytes, cudaMemcpyHostToDevice);
+            // a copy from pageable memory may still be under way when the call returns, in order with the legacy
+            // stream only: a step on a stream that does not wait for that one would read what was there before
+            if (e == cudaSuccess) e = cudaStreamSynchronize(cudaStreamLegacy);
             plan->dev = static_cast<Chunk*>(dev);
             if (e != cudaSuccess) {
                 if (dev) cudaFree(dev);

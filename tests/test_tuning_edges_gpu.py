@@ -1,11 +1,15 @@
 """Edges of the tuning operators on the GPU: stored codes bit by bit, rows and heads where a number runs out of its
 range, gradients that sit differently from their logits. Tolerances as derived in tests/test_tuning_ops_gpu.py."""
+import ctypes
+
 import pytest
 import torch
 
-from paperkiln_b200 import _capi  # noqa: F401
+from paperkiln_b200 import _capi
+from tests import pkt
 from tests import test_tuning_ops_gpu as ops
 from tests import tuning_ref as ref
+from tests.pkt import ptr, stream
 from tests.test_tuning_ops_gpu import HYPER, Many, f32, gen, pk  # noqa: F401
 
 pytestmark = pytest.mark.gpu
@@ -48,3 +52,23 @@ def test_stored_codes_are_those_of_the_step_in_fp32(pk, g_dtype, shift):  # noqa
         for what, (c, b), got_c, got_b in (("m", to_codes(m), s.m[i], s.ms[i]), ("v", to_codes(torch.sqrt(v), bits), s.v[i], s.vs[i])):
             assert torch.equal(b, got_b), what
             assert int((c != got_c).sum()) == 0, (what, n, int((c != got_c).sum()))
+
+
+def test_a_step_right_behind_its_plan_on_a_stream_of_its_own(pk):  # noqa: F811
+    """A table of several megabytes, and the step at once on a stream that waits for no other."""
+    count, n = 60000, 32
+    side = torch.cuda.Stream()
+    p0, g, m0, v0 = (torch.randn(count * n, device="cuda", generator=gen(i)) for i in range(4))
+    v0 = v0.square()
+    want = [t.clone() for t in (p0, m0, v0)]
+    pkt.check(pk.pk_adamw(stream(), ptr(want[0]), ptr(g), ptr(want[1]), ptr(want[2]), count * n, 1e-3, 0.9, 0.999, 1e-8, 0.1, 0.2, 0.01, None))
+    for _ in range(4):
+        p, m, v = p0.clone(), m0.clone(), v0.clone()
+        tensors = [_capi.AdamwTensor(p=p.data_ptr() + 4 * a, g=g.data_ptr() + 4 * a, m=m.data_ptr() + 4 * a, v=v.data_ptr() + 4 * a, n=n,
+                                     lr_mult=1.0, weight_decay=0.1) for a in range(0, count * n, n)]
+        torch.cuda.synchronize()
+        plan = _capi.AdamwPlan(tensors, 0, 32)
+        pkt.check(pk.pk_adamw_multi(ctypes.c_void_p(side.cuda_stream), plan.handle, 1e-3, 0.9, 0.999, 1e-8, 0.2, 0.01, 1))
+        side.synchronize()
+        plan.close()
+        assert all(torch.equal(a, b) for a, b in zip((p, m, v), want))
