@@ -398,12 +398,13 @@ qk_norm_rope_bwd_kernel(QkArgs a) {
 // dw += sum of the kind's partials, in a fixed order: a block owns 32 columns, its 32 warps take every
 // 32nd partial and are then added in ascending order.
 __global__ void __launch_bounds__(1024)
-qk_gain_grad_kernel(const float* __restrict__ partial, int nq, int nk, int dk, float* __restrict__ dwq, float* __restrict__ dwk) {
+qk_gain_grad_kernel(const float* partial, int nq, int nk, int dk, float* dwq, float* dwk) {
     __shared__ float red[32][33];
     const int c = blockIdx.x * 32 + threadIdx.x, n = blockIdx.y == 0 ? nq : nk;
     float* out = blockIdx.y == 0 ? dwq : dwk;
     if (blockIdx.y == 1) partial += static_cast<int64_t>(nq) * dk;
-    // launched while the backward still runs, whose partials it waits for here
+    // launched while the backward still runs, whose partials it waits for here (and so no __restrict__: what is written in
+    // this kernel's lifetime must be read coherently)
     asm volatile("griddepcontrol.wait;" ::: "memory");
     if (out == nullptr) return;
     float v = 0.0f;

@@ -1,5 +1,7 @@
-"""Host side of the tuning operators where it can go wrong without a word: the upload of an optimizer plan."""
+"""What the tuning operators promise to the hardware and to their callers, checked without a GPU: the upload of an optimizer
+plan, loads of kernels that start early."""
 import ctypes
+import re
 import subprocess
 from pathlib import Path
 
@@ -100,3 +102,30 @@ def test_a_plan_whose_upload_fails_leaves_nothing(plans):
     finally:
         plans.test_fail(0)
     assert plans.test_live() == 0
+
+
+def kernels(text):
+    """(name, parameters, body) of every kernel of a source file, comments left out."""
+    text = re.sub(r"//[^\n]*", "", text)
+    for head in re.finditer(r"__global__", text):
+        at = text.index("{", head.end())
+        sign, depth, end = text[head.end():at], 0, at
+        for end in range(at, len(text)):
+            depth += {"{": 1, "}": -1}.get(text[end], 0)
+            if depth == 0:
+                break
+        name = re.findall(r"(\w+)\s*\((?!\()", re.sub(r"__launch_bounds__\s*\((?:[^()]|\([^()]*\))*\)", "", sign))[0]
+        yield name, sign, text[at:end]
+
+
+def test_kernels_that_start_early_read_coherently():
+    """A kernel that is launched before its predecessor has ended lives while that one writes what it will read. `const
+    __restrict__` parameters allow loads that are defined only for data that nobody writes in a kernel's lifetime."""
+    early = []
+    for src in sorted(b.CSRC.glob("*.cu")):
+        for name, sign, body in kernels(src.read_text()):
+            if "griddepcontrol.wait" in body or "after_predecessor" in body:
+                early.append(name)
+                assert "__restrict__" not in sign, (src.name, name)
+                assert "__ldg" not in body and ".nc." not in body, (src.name, name)
+    assert {"token_logprob_bwd_kernel", "sweep_kernel", "preference_loss_kernel", "qk_gain_grad_kernel"} <= set(early)
