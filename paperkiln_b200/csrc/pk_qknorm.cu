@@ -316,7 +316,9 @@ __device__ __forceinline__ void backward_task(const QkArgs& a, const Kind& k, co
                 q2 = f2_fma(f2_mul(gv[j].odd[i], w[j].odd[i]), xv[j].odd[i], q2);
             }
         }
-        const float inv = rsqrtf(team_sum<LANES>(f2_sum(q1)) * inv_dk + a.eps);
+        // a team without a head or token holds zeros: with eps = 0 its root would be infinite, and 0 * inf in dw
+        float inv = rsqrtf(team_sum<LANES>(f2_sum(q1)) * inv_dk + a.eps);
+        if (F == ANY && !(token && h < heads)) inv = 0.0f;
         const uint64_t inv2 = f2_both(inv), k2 = f2_both(-team_sum<LANES>(f2_sum(q2)) * inv_dk * inv * inv);
 #pragma unroll
         for (int j = 0; j < PIECES; ++j) {

@@ -9,7 +9,7 @@ from paperkiln_b200 import _capi
 from tests import pkt
 from tests import test_tuning_ops_gpu as ops
 from tests import tuning_ref as ref
-from tests.pkt import ptr, stream
+from tests.pkt import dt, ptr, scratch, stream
 from tests.test_tuning_ops_gpu import HYPER, Many, f32, gen, pk  # noqa: F401
 
 pytestmark = pytest.mark.gpu
@@ -72,3 +72,34 @@ def test_a_step_right_behind_its_plan_on_a_stream_of_its_own(pk):  # noqa: F811
         side.synchronize()
         plan.close()
         assert all(torch.equal(a, b) for a, b in zip((p, m, v), want))
+
+
+# ---- q / k norms without an epsilon ------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("shape", [(5, 3, 2, 64), (7, 14, 2, 64), (1, 1, 1, 2), (3, 5, 3, 96), (9, 6, 1, 34), (1027, 14, 2, 64), (1025, 3, 1, 80),
+                                   (1501, 16, 2, 128)])
+def test_gain_gradients_without_epsilon(pk, dtype, shape):  # noqa: F811
+    """eps = 0 where a round of heads or a group of tokens is not full: places without a head add nothing to the gains'
+    gradients."""
+    T, Hq, Hkv, dk = shape
+    n_pos, hs = 50, ops.half_step(dtype)
+    q, gq = (torch.randn(T, Hq * dk, device="cuda", generator=gen(i)).to(dtype) for i in (1, 2))
+    k, gk = (torch.randn(T, Hkv * dk, device="cuda", generator=gen(i)).to(dtype) for i in (3, 4))
+    wq, wk = (1 + 0.3 * torch.randn(dk, device="cuda", generator=gen(i)) for i in (5, 6))
+    pos = torch.randint(0, n_pos, (T,), device="cuda", generator=gen(7)).to(torch.int32)
+    cs32 = ref.table(n_pos, dk, 1e4).float().cuda()
+    oq, ok, dq, dk_ = torch.empty_like(q), torch.empty_like(k), torch.empty_like(q), torch.empty_like(k)
+    dwq, dwk = torch.zeros(dk, device="cuda"), torch.zeros(dk, device="cuda")
+    buf = scratch(pk.pk_qk_norm_rope_bwd_scratch_bytes(T, Hq, Hkv, dk))
+    lq, lk = Hq * dk, Hkv * dk
+    pkt.check(pk.pk_qk_norm_rope_fwd(stream(), dt(q), ptr(q), lq, ptr(k), lk, ptr(wq), ptr(wk), ptr(oq), lq, ptr(ok), lk, T, Hq, Hkv, dk, Hq, Hkv,
+                                     0.0, ptr(pos), ptr(cs32), n_pos))
+    pkt.check(pk.pk_qk_norm_rope_bwd(stream(), dt(q), ptr(gq), lq, ptr(gk), lk, ptr(q), lq, ptr(k), lk, ptr(wq), ptr(wk), ptr(dq), lq, ptr(dk_), lk,
+                                     ptr(dwq), ptr(dwk), ptr(buf), T, Hq, Hkv, dk, Hq, Hkv, 0.0, ptr(pos), ptr(cs32), n_pos))
+    for x, g, w, H, y, dx, dw in ((q, gq, wq, Hq, oq, dq, dwq), (k, gk, wk, Hkv, ok, dk_, dwk)):
+        want, size = ref.qk_forward(x.double(), w.double(), H, cs32.double(), pos.long(), H, 0.0, sizes=True)
+        ops.within(y, want, hs * want.abs() + 2.0 ** -19 * size)
+        want, wdw, (size, wsize) = ref.qk_backward(g.double(), x.double(), w.double(), H, cs32.double(), pos.long(), H, 0.0)
+        ops.within(dx, want, hs * want.abs() + 2.0 ** -18 * size)
+        ops.within(dw, wdw, 2.0 ** -17 * wsize + 4 * ops.U * wdw.abs())
