@@ -513,7 +513,9 @@ sweep_kernel(const RowArgs a) {
             }
         };
         if (from < to) {
+            // the form goes by the row's maximum alone: res.y carries the 2^-r of the plain one
             if (base.plain && wide) give(std::true_type(), std::true_type());
+            else if (base.plain) give(std::true_type(), std::false_type());
             else if (wide) give(std::false_type(), std::true_type());
             else give(std::false_type(), std::false_type());
         }

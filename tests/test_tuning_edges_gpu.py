@@ -103,3 +103,41 @@ def test_gain_gradients_without_epsilon(pk, dtype, shape):  # noqa: F811
         want, wdw, (size, wsize) = ref.qk_backward(g.double(), x.double(), w.double(), H, cs32.double(), pos.long(), H, 0.0)
         ops.within(dx, want, hs * want.abs() + 2.0 ** -18 * size)
         ops.within(dw, wdw, 2.0 ** -17 * wsize + 4 * ops.U * wdw.abs())
+
+
+# ---- gradients that sit differently from their logits ------------------------------------------
+
+def raised(R, V, ld, offset, dtype, base, seed=0):
+    """Logits around `base`, as far as the type holds them apart."""
+    x, t = ops.make_logits(R, V, ld, offset, torch.float32, seed)
+    _, y = ops.strided(R, V, ld, offset, dtype)
+    y.copy_(x + base)
+    return y, t
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("V", [519, 5003, 40000])
+@pytest.mark.parametrize("base", [0.0, 12345.6, -1e5, 9e5, 3e6])
+def test_policy_gradient_of_another_alignment(pk, dtype, V, base):  # noqa: F811
+    """Where logits and gradient sit differently against 16 bytes the gradient has the bits that it has side by side, and
+    is right, whatever the rows' size."""
+    R, ld = 5, (V + 15) // 8 * 8
+    x, t = raised(R, V, ld, 0, dtype, base)
+    ti, adv = t.to(torch.int32), torch.randn(R, device="cuda", generator=gen(3))
+    loss, got = torch.empty(R, device="cuda"), []
+    for ldd, off in ((ld, 0), (ld + 3, 1), (V, 2)):
+        buf, dx = ops.strided(R, V, ldd, off, dtype)
+        pkt.check(pk.pk_policy_loss(stream(), dt(x), ptr(x), ld, ptr(ti), None, None, ptr(adv), None, 0.2, 0.2, 0.0, 1.0, ptr(loss), None, None,
+                                    ptr(dx), ldd, R, V, None))
+        got.append(dx.clone())
+        outside = torch.ones_like(buf, dtype=torch.bool)
+        outside[off:].as_strided((R, V), (ldd, 1))[:] = False
+        assert bool((buf[outside] == 7).all())
+    x64, g = x.double(), -adv.double()
+    _, lse = ref.logprob(x64, t)
+    want = ref.logprob_back(x64, t, lse, g)
+    p = torch.exp(x64 - lse[:, None])
+    lim = ops.half_step(dtype) * want.abs() + g.abs()[:, None] * (p * (2.0 ** -18 + 2.0 ** -21 * (x64 - lse[:, None]).abs()) + 2 * ops.U) + 1e-38
+    for dx in got:
+        ops.within(dx, want, lim)
+        assert torch.equal(dx, got[0])
