@@ -143,8 +143,8 @@ __device__ __forceinline__ float team_sum(float v) {
 }
 
 // A thread holds PIECES pieces of N elements of its head: piece j covers elements
-// (j * LANES + lane) * N. Lanes past dk, teams past the last head or token hold zeros, so that the
-// shuffles always take all lanes.
+// (j * LANES + lane) * N. Lanes past dk hold zeros, teams past the last head or token zeros or ones, so
+// that the shuffles always take all lanes.
 template <typename T, int N, int LANES, int PIECES>
 struct Place {
     int team, tl;
@@ -280,7 +280,13 @@ __device__ __forceinline__ void backward_task(const QkArgs& a, const Kind& k, co
     for (int u = 0; u < UU; ++u)
 #pragma unroll
         for (int j = 0; j < PIECES; ++j) {
-            if (F == ANY) xr[u][j] = gr[u][j] = make_uint4(0, 0, 0, 0);
+            if (F == ANY) {
+                // A team without a head or token holds x = 1 and g = 0, and so adds 0 to dw: with x = 0 and eps = 0 its root
+                // would be infinite, and 0 * inf. (The root set to 0 there instead: 191 -> 199 us at 65536 x 14 / 2 heads of 96.)
+                const uint32_t one = at.col(j) < a.dk ? (sizeof(T) == 2 ? 0x3f803f80u : 0x3f800000u) : 0u;
+                xr[u][j] = make_uint4(one, one, one, one);
+                gr[u][j] = make_uint4(0, 0, 0, 0);
+            }
             if (F != ANY || (token && h0 + u * k.step < heads && at.col(j) < a.dk)) {
                 xr[u][j] = Piece<T, N>::load_raw(x + u * hop + j * (LANES * N));
                 gr[u][j] = Piece<T, N>::load_raw(g + u * hop + j * (LANES * N));
@@ -316,9 +322,7 @@ __device__ __forceinline__ void backward_task(const QkArgs& a, const Kind& k, co
                 q2 = f2_fma(f2_mul(gv[j].odd[i], w[j].odd[i]), xv[j].odd[i], q2);
             }
         }
-        // a team without a head or token holds zeros: with eps = 0 its root would be infinite, and 0 * inf in dw
-        float inv = rsqrtf(team_sum<LANES>(f2_sum(q1)) * inv_dk + a.eps);
-        if (F == ANY && !(token && h < heads)) inv = 0.0f;
+        const float inv = rsqrtf(team_sum<LANES>(f2_sum(q1)) * inv_dk + a.eps);
         const uint64_t inv2 = f2_both(inv), k2 = f2_both(-team_sum<LANES>(f2_sum(q2)) * inv_dk * inv * inv);
 #pragma unroll
         for (int j = 0; j < PIECES; ++j) {
