@@ -367,7 +367,9 @@ int pk_fill(void* stream, int dtype, void* dst, float value, int64_t n);
  *
  * logp[i] = logits[i, t_i] - lse[i], lse[i] = log(sum_j exp(logits[i, j])), fp32. weight may be NULL
  * (every row counts). The backward writes dlogits[i, j] = dlogp[i] * ([j == t_i] - exp(logits[i, j] - lse[i]));
- * rows with dlogp[i] == 0 are written as zeros without their logits being read. */
+ * rows with dlogp[i] == 0 are written as zeros without their logits being read. Where |lse| is so large that its
+ * rounding to fp32 would show (from 64 on for fp32, 1024 for bf16) and it is the row's own, maximum and sum are taken
+ * from the row anew, at the cost of reading it again: a row of the type's lowest value alone is uniform. */
 int pk_token_logprob(void* stream, int dtype, const void* logits, int64_t ld, const int32_t* targets,
                      const float* weight, float* logp, float* lse, int64_t R, int64_t V, int32_t* status);
 int pk_token_logprob_bwd(void* stream, int dtype, const void* logits, int64_t ld, const int32_t* targets,

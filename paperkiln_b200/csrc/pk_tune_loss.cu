@@ -81,10 +81,10 @@ template <typename T> struct RowSplit {
     }
 };
 
-// dx[j] = g ([j == t] - exp(x_j - lse)): `threads` threads, of which this is `tid`, write one row. x and dx may be
+// dx[j] = g [j == t] - k exp(x_j - base): `threads` threads, of which this is `tid`, write one row. x and dx may be
 // the same row; they are read and written by the same thread, element by element or vector by vector.
 template <typename T>
-__device__ __forceinline__ void row_grad(const T* x, T* dx, int64_t V, int64_t t, float lse, float g, int64_t tid, int64_t threads) {
+__device__ __forceinline__ void row_grad(const T* x, T* dx, int64_t V, int64_t t, float base, float k, float g, int64_t tid, int64_t threads) {
     constexpr int N = Vec<T>::N;
     const RowSplit<T> sp(x, V);
     const bool wide = ((reinterpret_cast<uintptr_t>(x) ^ reinterpret_cast<uintptr_t>(dx)) & 15u) == 0;
@@ -97,7 +97,7 @@ __device__ __forceinline__ void row_grad(const T* x, T* dx, int64_t V, int64_t t
             const int64_t te = t - sp.head - i * N;
 #pragma unroll
             for (int e = 0; e < N; ++e) {
-                f[e] = ex2((f[e] - lse) * LOG2E) * -g;
+                f[e] = ex2((f[e] - base) * LOG2E) * -k;
                 if (te == e) f[e] += g;
             }
             Vec<T>::store(out + i * N, f);
@@ -106,7 +106,7 @@ __device__ __forceinline__ void row_grad(const T* x, T* dx, int64_t V, int64_t t
     const int64_t edge = wide ? sp.head + V - sp.tail0 : V;  // elements outside the vectors
     for (int64_t i = tid; i < edge; i += threads) {
         const int64_t c = !wide || i < sp.head ? i : sp.tail0 + i - sp.head;
-        float f = ex2((to_f32(x[c]) - lse) * LOG2E) * -g;
+        float f = ex2((to_f32(x[c]) - base) * LOG2E) * -k;
         if (c == t) f += g;
         dx[c] = from_f32<T>(f);
     }
@@ -118,28 +118,6 @@ __device__ __forceinline__ void row_zero(T* dx, int64_t V, int64_t tid, int64_t 
     for (int64_t i = tid; i < sp.nv; i += threads) *reinterpret_cast<uint4*>(dx + sp.head + i * N) = make_uint4(0, 0, 0, 0);
     for (int64_t c = tid; c < sp.head; c += threads) dx[c] = from_f32<T>(0.0f);
     for (int64_t c = sp.tail0 + tid; c < V; c += threads) dx[c] = from_f32<T>(0.0f);
-}
-
-template <typename T>
-__global__ void __launch_bounds__(512)
-token_logprob_bwd_kernel(const T* logits, int64_t ld, const int32_t* targets, const float* lse,
-                         const float* dlogp, T* dlogits, int64_t ldd, int64_t R, int64_t V, int32_t* status) {
-    // gridDim.y blocks share a row. Last rows first: the pass that took the log-probabilities has left them in L2.
-    const int64_t tid = blockIdx.y * blockDim.x + threadIdx.x, threads = gridDim.y * blockDim.x;
-    after_predecessor();
-    for (int64_t row = R - 1 - blockIdx.x; row >= 0; row -= gridDim.x) {
-        float g = dlogp[row];
-        T* dx = dlogits + row * ldd;
-        if (g != 0.0f) {
-            const int64_t t = targets[row];
-            if (t >= 0 && t < V) {
-                row_grad(logits + row * ld, dx, V, t, lse[row], g, tid, threads);
-                continue;
-            }
-            if (tid == 0 && status) atomicOr(status, PK_ERR_INDEX);
-        }
-        row_zero(dx, V, tid, threads);
-    }
 }
 
 // x - (m + log(s)) and m + log(s), each as if rounded once: log(s) = k log(2) + log(f) with f in [sqrt(1/2), sqrt(2)),
@@ -175,6 +153,67 @@ struct LogSum {
         return b + left;
     }
 };
+
+// The same for a row whose lse has few bits behind the point. exp(x - lse) is off by the rounding of lse, |lse| 2^-24
+// (by a factor of V in a row of the type's lowest value alone), so maximum and sum are found again from the row, and
+// serve where the lse is theirs (one over more words than the row holds is taken as it is). A block reads all of the row
+// before it writes any, so one block has it to itself. From 64 on for fp32 (below, at most 2^-18, what an exponential
+// may be off), from 1024 for bf16 (2^-14, against its own rounding of 2^-9); ordinary rows never come here.
+template <typename T>
+__device__ __noinline__ void row_grad_large(const T* x, T* dx, int64_t V, int64_t t, float lse, float g) {
+    __shared__ float red[32];
+    if (blockIdx.y != 0) return;
+    constexpr int N = Vec<T>::N;
+    const RowSplit<T> sp(x, V);
+    const int tid = threadIdx.x, threads = blockDim.x;
+    const int64_t edge = sp.head + V - sp.tail0;
+    float m = -INFINITY, s = 0.0f;
+    for (int64_t i = tid; i < sp.nv; i += threads) {
+        float f[N];
+        Vec<T>::load(x + sp.head + i * N, f);
+#pragma unroll
+        for (int e = 0; e < N; ++e) m = fmaxf(m, f[e]);
+    }
+    for (int64_t i = tid; i < edge; i += threads) m = fmaxf(m, to_f32(x[i < sp.head ? i : sp.tail0 + i - sp.head]));
+    m = block_max(m, red);
+    for (int64_t i = tid; i < sp.nv; i += threads) {
+        float f[N], part = 0.0f;
+        Vec<T>::load(x + sp.head + i * N, f);
+#pragma unroll
+        for (int e = 0; e < N; ++e) part += expf(f[e] - m);
+        s += part;
+    }
+    for (int64_t i = tid; i < edge; i += threads) s += expf(to_f32(x[i < sp.head ? i : sp.tail0 + i - sp.head]) - m);
+    s = block_sum(s, red);
+    const float own = LogSum({m, s}).lse();
+    const bool mine = fabsf(own - lse) <= fminf(fabsf(lse) * 0x1p-22f, 1e38f);  // two to four steps of fp32; not an infinite one
+    row_grad(x, dx, V, t, mine ? m : lse, mine ? g / s : g, g, tid, threads);
+    __syncthreads();  // red is free for the block's next such row
+}
+
+template <typename T>
+__global__ void __launch_bounds__(512, 4)  // 32 registers at most: large rows must not cost the others their residency
+token_logprob_bwd_kernel(const T* logits, int64_t ld, const int32_t* targets, const float* lse,
+                         const float* dlogp, T* dlogits, int64_t ldd, int64_t R, int64_t V, int32_t* status) {
+    // gridDim.y blocks share a row. Last rows first: the pass that took the log-probabilities has left them in L2.
+    const int64_t tid = blockIdx.y * blockDim.x + threadIdx.x, threads = gridDim.y * blockDim.x;
+    after_predecessor();
+    for (int64_t row = R - 1 - blockIdx.x; row >= 0; row -= gridDim.x) {
+        float g = dlogp[row];
+        T* dx = dlogits + row * ldd;
+        if (g != 0.0f) {
+            const int64_t t = targets[row];
+            if (t >= 0 && t < V) {
+                const float l = lse[row];
+                if (fabsf(l) >= (sizeof(T) == 2 ? 1024.0f : 64.0f)) row_grad_large(logits + row * ld, dx, V, t, l, g);
+                else row_grad(logits + row * ld, dx, V, t, l, g, g, tid, threads);
+                continue;
+            }
+            if (tid == 0 && status) atomicOr(status, PK_ERR_INDEX);
+        }
+        row_zero(dx, V, tid, threads);
+    }
+}
 
 struct PolicyArgs {
     const int32_t* targets;

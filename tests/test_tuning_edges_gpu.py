@@ -141,3 +141,60 @@ def test_policy_gradient_of_another_alignment(pk, dtype, V, base):  # noqa: F811
     for dx in got:
         ops.within(dx, want, lim)
         assert torch.equal(dx, got[0])
+
+
+# ---- gradients of log-probabilities whose sum has few bits left --------------------------------
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("V", [37, 2056, 40000])
+@pytest.mark.parametrize("R", [4, 3000])
+def test_logprob_gradient_of_large_rows(pk, dtype, V, R):  # noqa: F811
+    """exp(x - lse) with an lse of 24 bits is off by up to |lse| 2^-24, a row of the lowest value alone by a factor of V:
+    such rows get their probabilities from the row itself. Few rows (several blocks to a row) and many, apart and in place."""
+    if R > 4 and V > 10000:
+        R = 700
+    low = torch.finfo(dtype).min
+    x, t = raised(R, V, V, 0, dtype, 0.0)
+    for i, base in enumerate((1e5, -2e6, 300.0, -5000.0, 70.0, -60.0, 4e4, 0.0)):
+        x[i::11] += base
+    x[8::11] = low            # nothing but masked words: uniform
+    x[0] = low
+    x[1, 1::2] = low          # and some of a row's
+    x[R - 1, ::3] = -float("inf")
+    t[1] = 0
+    t[R - 1] = 1
+    ti, g = t.to(torch.int32), torch.randn(R, device="cuda", generator=gen(9))
+    logp, lse = torch.empty(R, device="cuda"), torch.empty(R, device="cuda")
+    pkt.check(pk.pk_token_logprob(stream(), dt(x), ptr(x), V, ptr(ti), None, ptr(logp), ptr(lse), R, V, None))
+    x64, g64 = x.double(), g.double()
+    top = x64.amax(1, keepdim=True)
+    e = torch.exp(x64 - top)
+    p = e / e.sum(1, keepdim=True)
+    want = -g64[:, None] * p
+    want[torch.arange(R, device="cuda"), t] += g64
+    far = (x64 - top).clamp(min=-1e4).abs() + torch.log(torch.tensor(float(V)))
+    # below 64 (fp32) and 1024 (bf16) the lse serves as it is: half a step of it is 2^-18 (2^-14, of the rounding to come 2^-5)
+    rel = 2.0 ** -17 + 2.0 ** -21 * far + (2.0 ** -18 if dtype == torch.float32 else 2.0 ** -14)
+    lim = ops.half_step(dtype) * want.abs() + g64.abs()[:, None] * (p * rel + 2 * ops.U) + 1e-38
+    dx = torch.full_like(x, 3.0)
+    call = lambda out: pkt.check(pk.pk_token_logprob_bwd(stream(), dt(x), ptr(x), V, ptr(ti), ptr(lse), ptr(g), ptr(out), V, R, V, None))  # noqa: E731
+    call(dx)
+    ops.within(dx, want, lim)
+    call(x)
+    assert torch.equal(dx, x)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_logprob_gradient_under_a_sum_over_more_words(pk, dtype):  # noqa: F811
+    """An lse that is not this row's own (the words of a row lie in two tensors, say) is taken as it is given."""
+    R, V = 6, 1000
+    x, t = raised(R, V, V, 0, dtype, 0.0)
+    x += 3000.0
+    ti, g = t.to(torch.int32), torch.randn(R, device="cuda", generator=gen(9))
+    lse = (torch.logsumexp(x.double(), 1) + 1.5).float()
+    dx = torch.empty_like(x)
+    pkt.check(pk.pk_token_logprob_bwd(stream(), dt(x), ptr(x), V, ptr(ti), ptr(lse), ptr(g), ptr(dx), V, R, V, None))
+    want = ref.logprob_back(x.double(), t, lse.double(), g.double())
+    p = torch.exp(x.double() - lse.double()[:, None])
+    far = (x.double() - lse.double()[:, None]).abs()
+    ops.within(dx, want, ops.half_step(dtype) * want.abs() + g.double().abs()[:, None] * (p * (2.0 ** -18 + 2.0 ** -21 * far) + 2 * ops.U) + 1e-38)
