@@ -393,7 +393,8 @@ int pk_preference_loss(void* stream, const float* logp, const float* ref_logp, c
  *     row_loss = w * (-min(r A, clamp(r, 1 - clip_lo, 1 + clip_hi) A) + kl_coef * (exp(u) - u - 1))
  *     dlogits  = grad_scale * d row_loss / d logits
  * old_logp == NULL: the rows were sampled from this very policy (r = 1, its gradient counted);
- * ref_logp == NULL: no KL term (kl is then 0); weight == NULL: 1. logp and kl (= exp(u) - u - 1) may be
+ * ref_logp == NULL: no KL term (kl is then 0); kl_coef == 0 leaves the term out of loss and gradient, an advantage of 0
+ * the ratio's, even where e^u or r is past the type's range; weight == NULL: 1. logp and kl (= exp(u) - u - 1) may be
  * NULL; dlogits == NULL: the loss alone. On a clipping bound the unclipped branch counts. */
 int pk_policy_loss(void* stream, int dtype, const void* logits, int64_t ld, const int32_t* targets,
                    const float* old_logp, const float* ref_logp, const float* advantage, const float* weight,

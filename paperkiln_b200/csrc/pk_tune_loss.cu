@@ -224,11 +224,11 @@ struct PolicyArgs {
 };
 
 // e^u - u - 1 without the cancellation near zero: its series there (the next term is below 2^-24 of
-// the first for |u| < 0.1), expm1 elsewhere.
+// the first for |u| < 0.1), expm1 elsewhere, alone where u is below its last bit (and may be infinite).
 __device__ __forceinline__ float kl_term(float u) {
     if (fabsf(u) < 0.1f)
         return u * u * (0.5f + u * (1.0f / 6 + u * (1.0f / 24 + u * (1.0f / 120 + u * (1.0f / 720 + u * (1.0f / 5040))))));
-    return expm1f(u) - u;
+    return u > 64.0f ? expm1f(u) : expm1f(u) - u;
 }
 // What the loss takes from a row besides its logits: fetched before the row's reduction, so that the
 // fetch does not stand behind it.
@@ -243,7 +243,8 @@ struct PolicyRow {
 };
 // d loss / d logp of a row, for every thread that asks; one of them writes the row's loss.
 __device__ __forceinline__ float policy_row(const PolicyArgs& a, int64_t row, const PolicyRow& q, float logp, bool writer) {
-    const float r = a.old_logp ? expf(logp - q.old) : (logp == logp ? 1.0f : logp);
+    float r = a.old_logp ? expf(logp - q.old) : (logp == logp ? 1.0f : logp);
+    if (q.adv == 0.0f && r == INFINITY) r = 1.0f;  // a ratio past the type's range counts for nothing all the same
     const float free_ = r * q.adv, held = fminf(fmaxf(r, a.lo), a.hi) * q.adv;
     float loss = -held, g = 0.0f, kl = 0.0f;
     if (free_ <= held) loss = g = -free_;
@@ -251,8 +252,10 @@ __device__ __forceinline__ float policy_row(const PolicyArgs& a, int64_t row, co
     if (a.ref_logp) {
         const float u = q.ref - logp;
         kl = kl_term(u);
-        loss += a.kl_coef * kl;
-        g -= a.kl_coef * expm1f(u);
+        if (a.kl_coef != 0.0f) {  // without it e^u may be infinite
+            loss += a.kl_coef * kl;
+            g -= a.kl_coef * expm1f(u);
+        }
     }
     if (writer) {
         a.row_loss[row] = q.w * loss;

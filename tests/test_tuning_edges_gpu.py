@@ -198,3 +198,35 @@ def test_logprob_gradient_under_a_sum_over_more_words(pk, dtype):  # noqa: F811
     p = torch.exp(x.double() - lse.double()[:, None])
     far = (x.double() - lse.double()[:, None]).abs()
     ops.within(dx, want, ops.half_step(dtype) * want.abs() + g.double().abs()[:, None] * (p * (2.0 ** -18 + 2.0 ** -21 * far) + 2 * ops.U) + 1e-38)
+
+
+# ---- terms of the policy loss that do not count ------------------------------------------------
+
+def test_policy_terms_of_coefficient_zero(pk):  # noqa: F811
+    """A KL coefficient of zero and an advantage of zero leave their terms out, also where e^u or the ratio passes the
+    type's range (a reference or an old policy that had all but excluded the word): 0 * inf is no loss."""
+    V = 64
+    x = torch.randn(4, V, device="cuda", generator=gen(2))
+    t = torch.tensor([1, 2, 3, 4], dtype=torch.int32, device="cuda")
+    lp = ref.logprob(x.double(), t.long())[0].float()
+    loss, kl, dx = torch.empty(4, device="cuda"), torch.empty(4, device="cuda"), torch.empty(4, V, device="cuda")
+
+    def run(old, refp, adv, c):
+        pkt.check(pk.pk_policy_loss(stream(), 0, ptr(x), V, ptr(t), ptr(old), ptr(refp), ptr(adv), None, 0.2, 0.2, c, 1.0, ptr(loss), None,
+                                    ptr(kl), ptr(dx), V, 4, V, None))
+        return loss.clone(), dx.clone()
+
+    adv = torch.tensor([1.0, -1.0, 0.5, 0.0], device="cuda")
+    want = run(lp, None, adv, 0.0)
+    got = run(lp, lp + torch.tensor([100.0, 200.0, float("inf"), 1.0], device="cuda"), adv, 0.0)
+    assert all(torch.equal(a, b) for a, b in zip(want, got))
+    assert kl[:3].tolist() == [float("inf")] * 3   # still told
+    # the ratio e^200 counts for nothing with an advantage of 0; the KL term does
+    none = torch.zeros(4, device="cuda")
+    a = run(lp - 200.0, lp + 0.1, none, 0.1)
+    b = run(lp, lp + 0.1, none, 0.1)
+    assert all(torch.equal(u, v) and bool(torch.isfinite(u).all()) for u, v in zip(a, b)) and bool((a[1] != 0).any())
+    a = run(lp - 200.0, None, none, 0.0)
+    assert not a[0].any() and not a[1].any()
+    x[1, 5] = float("nan")   # a row that holds NaN stays one
+    assert torch.isnan(run(lp, None, none, 0.0)[0]).tolist() == [False, True, False, False]
