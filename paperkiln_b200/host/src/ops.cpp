@@ -930,6 +930,7 @@ void read_rows(const Tensor& t, std::vector<float>* out) {
 // Targets of rows that count; the others may hold anything (-100 is usual).
 void check_targets(const std::vector<int>& targets, const std::vector<float>& weight, size_t R, size_t V) {
     if (targets.size() != R) throw std::runtime_error("one target per row");
+    if (!weight.empty() && weight.size() != R) throw std::runtime_error("one weight per row");
     for (size_t i = 0; i < R; ++i)
         if ((weight.empty() || weight[i] != 0.0f) && (targets[i] < 0 || static_cast<size_t>(targets[i]) >= V))
             throw std::runtime_error("target out of range");

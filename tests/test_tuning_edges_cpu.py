@@ -1,5 +1,5 @@
 """What the tuning operators promise to the hardware and to their callers, checked without a GPU: the upload of an optimizer
-plan, loads of kernels that start early."""
+plan, loads of kernels that start early, row weights of the C++ operators."""
 import ctypes
 import re
 import subprocess
@@ -129,3 +129,46 @@ def test_kernels_that_start_early_read_coherently():
                 assert "__restrict__" not in sign, (src.name, name)
                 assert "__ldg" not in body and ".nc." not in body, (src.name, name)
     assert {"token_logprob_bwd_kernel", "sweep_kernel", "preference_loss_kernel", "qk_gain_grad_kernel"} <= set(early)
+
+
+# ---- the C++ operators -------------------------------------------------------------------------
+
+WEIGHTS = r'''
+#include <cstdio>
+#include <functional>
+#include <stdexcept>
+#include <string>
+#include "microtorch/ops.hpp"
+using namespace microtorch;
+int main() {
+    Var h = make_var(Matrix(5, 4, 0.5f), false), W = make_var(Matrix(4, 7, 0.5f), false);
+    const std::vector<int> targets = {1, 2, -100, 3, -100};
+    const std::vector<float> rows(5, 1.0f), few(2, 1.0f), many(6, 0.0f);
+    ops::PolicyTerms policy;
+    ops::PreferenceTerms pref;
+    policy.advantage = rows;
+    pref.seq = {0, 2, 5};
+    int bad = 0;
+    for (const auto& w : {few, many}) {
+        policy.weight = pref.weight = w;
+        const std::function<void()> calls[] = {[&] { ops::linear_token_logprob(h, W, false, targets, w); },
+                                               [&] { ops::linear_policy_loss(h, W, false, targets, policy); },
+                                               [&] { ops::linear_preference_loss(h, W, false, targets, pref); }};
+        for (const auto& call : calls) {
+            std::string said = "nothing";
+            try { call(); } catch (const std::exception& e) { said = e.what(); }
+            if (said.find("one weight per row") == std::string::npos) { std::printf("%zu weights: %s\n", w.size(), said.c_str()); ++bad; }
+        }
+    }
+    return bad;
+}
+'''
+
+
+def test_weights_of_another_length_are_refused_before_they_are_read(tmp_path):
+    (tmp_path / "weights.cpp").write_text(WEIGHTS)
+    exe = tmp_path / "weights"
+    subprocess.run([b._host_cxx(), "-O1", "-std=c++17", "-I", str(b.INCLUDE), "-I", str(b.HOST / "include"), str(tmp_path / "weights.cpp"), "-o",
+                    str(exe), "-L", str(b.PKG), "-lmicrotorch", "-lpk", f"-Wl,-rpath,{b.PKG}"], check=True)
+    r = subprocess.run([str(exe)], capture_output=True, text=True, timeout=120)
+    assert r.returncode == 0, r.stdout + r.stderr
