@@ -65,7 +65,8 @@ void set_error(const char*, ...) {}
 
 @pytest.fixture(scope="module")
 def plans(tmp_path_factory):
-    """The optimizer's entries over that runtime, from this tree's source."""
+    """The optimizer's entries over that runtime, from this tree's source. (Bound to it, not to a runtime that another
+    library of the process has brought.)"""
     at = tmp_path_factory.mktemp("plans")
     src, obj = b.CSRC / "pk_adamw_multi.cu", b.OBJ / "pk_adamw_multi.o"
     if not b._newer(obj, [src, *b.CSRC.glob("*.cuh"), *b.INCLUDE.glob("*.h")]):
@@ -73,7 +74,7 @@ def plans(tmp_path_factory):
         subprocess.run([b._nvcc(), "-ccbin", b._host_cxx(), *b.NVCC_FLAGS, "-c", str(src), "-o", str(obj)], check=True)
     (at / "runtime.cpp").write_text(RUNTIME)
     cuda = Path(b._nvcc()).resolve().parent.parent / "include"
-    subprocess.run([b._host_cxx(), "-shared", "-fPIC", "-std=c++17", "-I", str(cuda), "-o", str(at / "plans.so"), str(at / "runtime.cpp"),
+    subprocess.run([b._host_cxx(), "-shared", "-fPIC", "-std=c++17", "-Wl,-Bsymbolic", "-I", str(cuda), "-o", str(at / "plans.so"), str(at / "runtime.cpp"),
                     str(obj)], check=True)
     return ctypes.CDLL(str(at / "plans.so"))
 
