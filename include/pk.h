@@ -216,11 +216,12 @@ int pk_gemm_rope(void* stream, int trans_b, int64_t M, int64_t N, int64_t K, con
  * kind. The rotation is that of pk_rope (interleaved pairs, the same table, positions outside
  * [0, n_pos) are clamped) and applies to the first rot_q / rot_k heads; with both 0, pos and cos_sin
  * may be NULL. Norm and rotation are fp32, the result is rounded once. Outputs may be the inputs
- * themselves (same pointer and stride: in place); any other overlap is not allowed. Any even
+ * themselves (same pointer and stride: in place); any other overlap is refused (column ranges of one buffer are apart when
+ * they are within the row stride, with two strides within the greatest common divisor of both). Any even
  * head_dim up to 256, any strides and alignment (16-byte aligned rows take wide accesses).
  * The backward takes the upstream gradients dqo / dko and the inputs q / k of the forward (nothing
  * else is saved: the norm is recomputed from the row it reads anyway) and writes dq / dk, which may
- * be dqo / dko; dwq and dwk are ACCUMULATED (+=), each may be NULL. Replaces ops::rmsnorm per head
+ * be dqo / dko or q / k; dwq and dwk are ACCUMULATED (+=), each may be NULL. Replaces ops::rmsnorm per head
  * and ops::apply_rope (src/ops.cpp:426-537), which the reference's blocks call one after the
  * other on whole rows and on one head. */
 int pk_qk_norm_rope_fwd(void* stream, int dtype, const void* q, int64_t ldq, const void* k, int64_t ldk,

@@ -13,6 +13,7 @@
 // and one token (of several tokens where a token has fewer heads than the warp has teams): U heads per
 // team, all loaded before the first is computed, with the rotation table's row and the gains in registers.
 #include <algorithm>
+#include <numeric>
 #include <type_traits>
 
 #include "pk_common.cuh"
@@ -511,6 +512,25 @@ bool rows_aligned(const void* p, int64_t ld, int dtype) {
     return aligned16(p) && static_cast<size_t>(ld) * dtype_size(dtype) % 16 == 0;
 }
 
+// T rows of a kind of heads.
+struct Rows {
+    const void* p;
+    int64_t ld, cols;
+};
+// Whether rows of a and b share memory. Two column ranges of one buffer span the same memory and do not, when they stay
+// apart within the rows' stride (of two strides, within their common measure).
+bool meet(const Rows& a, const Rows& b, int64_t T, size_t es) {
+    if (a.cols == 0 || b.cols == 0) return false;
+    const uintptr_t pa = reinterpret_cast<uintptr_t>(a.p), pb = reinterpret_cast<uintptr_t>(b.p);
+    const uintptr_t na = static_cast<uintptr_t>((T - 1) * a.ld + a.cols) * es, nb = static_cast<uintptr_t>((T - 1) * b.ld + b.cols) * es;
+    if (pa + na <= pb || pb + nb <= pa) return false;
+    if (T == 1) return true;
+    const uintptr_t m = static_cast<uintptr_t>(std::gcd(a.ld, b.ld)) * es, ca = a.cols * es, cb = b.cols * es;
+    const uintptr_t d = pb >= pa ? (pb - pa) % m : (m - (pa - pb) % m) % m;  // where b starts in a's stride
+    return !(d >= ca && d + cb <= m);
+}
+bool same(const Rows& a, const Rows& b) { return a.p == b.p && a.ld == b.ld; }
+
 }  // namespace
 }  // namespace pk
 
@@ -541,6 +561,15 @@ int pk_qk_norm_rope_fwd(void* stream, int dtype, const void* q, int64_t ldq, con
     const bool turn = rot_q + rot_k > 0;
     PK_REQUIRE(!turn || (pos && cos_sin && n_pos > 0), "the rotation needs positions and a table");
     PK_REQUIRE((q != qo || ldq == ldqo) && (k != ko || ldk == ldko), "in place needs equal row strides");
+    {
+        const size_t es = dtype_size(dtype);
+        const Rows in[2] = {{q, ldq, cq}, {k, ldk, ck}}, out[2] = {{qo, ldqo, cq}, {ko, ldko, ck}};
+        for (int r = 0; r < 2; ++r) {
+            PK_REQUIRE(same(out[r], in[r]) || !meet(out[r], in[r], T, es), "an output overlaps its input");
+            PK_REQUIRE(!meet(out[r], in[1 - r], T, es), "an output overlaps the input of the other kind");
+        }
+        PK_REQUIRE(!meet(out[0], out[1], T, es), "the outputs overlap");
+    }
     QkArgs a{};
     a.kind[0] = {q, nullptr, qo, ldq, 0, ldqo, wq, Hq, rot_q, 0, 0, 0, 0, 0};
     a.kind[1] = {k, nullptr, ko, ldk, 0, ldko, wk, Hkv, rot_k, 0, 0, 0, 0, 0};
@@ -581,6 +610,16 @@ int pk_qk_norm_rope_bwd(void* stream, int dtype, const void* dqo, int64_t lddqo,
     const bool gains = dwq != nullptr || dwk != nullptr;
     PK_REQUIRE(!gains || scratch, "the gains' gradients need scratch");
     PK_REQUIRE(!gains || dwq != dwk, "the two gains' gradients must be two buffers");
+    {
+        const size_t es = dtype_size(dtype);
+        const Rows in[2] = {{q, ldq, cq}, {k, ldk, ck}}, up[2] = {{dqo, lddqo, cq}, {dko, lddko, ck}}, out[2] = {{dq, lddq, cq}, {dk, lddk, ck}};
+        for (int r = 0; r < 2; ++r) {
+            PK_REQUIRE((same(out[r], in[r]) || !meet(out[r], in[r], T, es)) && (same(out[r], up[r]) || !meet(out[r], up[r], T, es)),
+                       "an output overlaps its input");
+            PK_REQUIRE(!meet(out[r], in[1 - r], T, es) && !meet(out[r], up[1 - r], T, es), "an output overlaps an input of the other kind");
+        }
+        PK_REQUIRE(!meet(out[0], out[1], T, es), "the outputs overlap");
+    }
     QkArgs a{};
     a.kind[0] = {q, dqo, dq, ldq, lddqo, lddq, wq, Hq, rot_q, 0, 0, 0, 0, 0};
     a.kind[1] = {k, dko, dk, ldk, lddko, lddk, wk, Hkv, rot_k, 0, 0, 0, 0, 0};

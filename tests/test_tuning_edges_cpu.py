@@ -1,11 +1,12 @@
 """What the tuning operators promise to the hardware and to their callers, checked without a GPU: the upload of an optimizer
-plan, loads of kernels that start early, row weights of the C++ operators."""
+plan, loads of kernels that start early, row weights of the C++ operators, overlaps of the head norms."""
 import ctypes
 import re
 import subprocess
 from pathlib import Path
 
 import pytest
+import torch
 
 from paperkiln_b200 import _capi
 from paperkiln_b200 import build as b
@@ -173,3 +174,77 @@ def test_weights_of_another_length_are_refused_before_they_are_read(tmp_path):
                     str(exe), "-L", str(b.PKG), "-lmicrotorch", "-lpk", f"-Wl,-rpath,{b.PKG}"], check=True)
     r = subprocess.run([str(exe)], capture_output=True, text=True, timeout=120)
     assert r.returncode == 0, r.stdout + r.stderr
+
+
+# ---- overlaps of the head norms ----------------------------------------------------------------
+
+BASE, FAR = 1 << 20, 1 << 30   # addresses that nothing reads: every call below is refused, or has no GPU to run on
+
+
+def address(base, elements, size):
+    return ctypes.c_void_p(base + elements * size)
+
+
+@pytest.fixture(scope="module")
+def pk():
+    return _capi.libpk()
+
+
+def forward(pk, q, k, qo, ko, size=4, T=3, Hq=4, Hkv=2, dk=16):
+    """q, k, qo, ko: (base, first element, row stride). True when the call is refused for an overlap."""
+    at = [(address(base, first, size), ld) for base, first, ld in (q, k, qo, ko)]
+    w = ctypes.c_void_p(FAR * 3)
+    rc = pk.pk_qk_norm_rope_fwd(None, 0 if size == 4 else 1, *at[0], *at[1], w, w, *at[2], *at[3], T, Hq, Hkv, dk, 0, 0, 1e-6, None, None, 0)
+    assert rc != 0   # no GPU here
+    return rc == 1 and b"overlap" in pk.pk_last_error()
+
+
+def backward(pk, dqo, dko, q, k, dq, dk_, size=4, T=3):
+    at = [(address(base, first, size), ld) for base, first, ld in (dqo, dko, q, k, dq, dk_)]
+    w = ctypes.c_void_p(FAR * 3)
+    rc = pk.pk_qk_norm_rope_bwd(None, 0 if size == 4 else 1, *at[0], *at[1], *at[2], *at[3], w, w, *at[4], *at[5], None, None, None, T, 4, 2, 16, 0, 0,
+                                1e-6, None, None, 0)
+    assert rc != 0
+    return rc == 1 and b"overlap" in pk.pk_last_error()
+
+
+@pytest.mark.skipif(torch.cuda.is_available(), reason="the calls that are let through name addresses without memory")
+@pytest.mark.parametrize("size", [2, 4])
+def test_head_norms_refuse_outputs_inside_their_inputs(pk, size):
+    q, k, qo, ko = (BASE, 0, 64), (2 * BASE, 0, 32), (FAR, 0, 64), (FAR + BASE, 0, 32)
+    f = lambda **o: forward(pk, **({"q": q, "k": k, "qo": qo, "ko": ko} | o), size=size)  # noqa: E731
+    assert not f()
+    assert not f(qo=q, ko=k)                                   # in place
+    assert not f(qo=q) and not f(ko=k)
+    assert f(qo=(BASE, 16, 64))                                # one head on: another team reads what this one writes
+    assert f(qo=(BASE, 64, 64))                                # one row on
+    assert f(qo=(BASE, 2 * 64 + 63, 64))                       # the last element of q alone
+    assert not f(qo=(BASE, 3 * 64, 64))                        # right behind it
+    assert f(qo=(2 * BASE, 0, 64)) and f(ko=q)                 # over the other kind
+    assert f(ko=(FAR, 48, 32))                                 # the outputs over each other
+    # column ranges of one packed projection: q | k | free, rows of 160
+    q, k = (BASE, 0, 160), (BASE, 64, 160)
+    g = lambda **o: forward(pk, **({"q": q, "k": k, "qo": qo, "ko": ko} | o), size=size)  # noqa: E731
+    assert not g() and not g(qo=q, ko=k)
+    assert not g(qo=(BASE, 96, 160)) and not g(ko=(BASE, 96, 160))
+    assert g(qo=(BASE, 97, 160))                               # reaches the next row's queries
+    assert g(qo=(BASE, 95, 160))                               # starts at the keys' end
+    assert not g(qo=(BASE, 160 + 96, 160))                     # a row further down the same columns
+    assert g(ko=(BASE, 160 + 80, 160))
+    # rows of another stride: apart when the columns are, in the strides' common measure
+    assert not g(qo=(BASE, 96, 320)) and g(qo=(BASE, 90, 320)) and g(qo=(BASE, 96, 176))
+    assert not forward(pk, (BASE, 0, 64), (2 * BASE, 0, 32), (BASE, 64, 80), ko, size=size, T=1)
+
+
+@pytest.mark.skipif(torch.cuda.is_available(), reason="the calls that are let through name addresses without memory")
+@pytest.mark.parametrize("size", [2, 4])
+def test_head_norm_gradients_refuse_outputs_inside_their_inputs(pk, size):
+    at = {"dqo": (BASE, 0, 64), "dko": (2 * BASE, 0, 32), "q": (3 * BASE, 0, 64), "k": (4 * BASE, 0, 32), "dq": (FAR, 0, 64),
+          "dk_": (FAR + BASE, 0, 32)}
+    f = lambda **o: backward(pk, **(at | o), size=size)  # noqa: E731
+    assert not f() and not f(dq=at["dqo"], dk_=at["dko"])
+    assert not f(dq=at["q"], dk_=at["k"])                      # every thread reads its elements before it writes them
+    assert f(dq=(BASE, 16, 64)) and f(dq=(3 * BASE, 16, 64)) and f(dk_=(2 * BASE, 32, 32)) and f(dk_=(4 * BASE, 1, 32))
+    assert f(dq=(4 * BASE, 0, 64)) and f(dk_=at["dqo"]) and f(dk_=at["q"]) and f(dk_=(FAR, 0, 64))
+    packed = {"dqo": (BASE, 0, 160), "dko": (BASE, 64, 160), "dq": (BASE, 0, 160), "dk_": (BASE, 64, 160)}
+    assert not f(**packed) and not f(**(packed | {"dk_": (BASE, 96, 160)})) and f(**(packed | {"dk_": (BASE, 60, 160)}))

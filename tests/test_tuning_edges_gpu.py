@@ -230,3 +230,21 @@ def test_policy_terms_of_coefficient_zero(pk):  # noqa: F811
     assert not a[0].any() and not a[1].any()
     x[1, 5] = float("nan")   # a row that holds NaN stays one
     assert torch.isnan(run(lp, None, none, 0.0)[0]).tolist() == [False, True, False, False]
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("shape", [(37, 14, 2, 64), (130, 3, 1, 80), (1027, 16, 4, 128)])
+def test_head_norm_gradients_over_the_inputs(pk, dtype, shape):  # noqa: F811
+    """dq / dk written over q / k: the same bits as elsewhere."""
+    T, Hq, Hkv, dk = shape
+    lq, lk = Hq * dk, Hkv * dk
+    q, gq = (torch.randn(T, lq, device="cuda", generator=gen(i)).to(dtype) for i in (1, 2))
+    k, gk = (torch.randn(T, lk, device="cuda", generator=gen(i)).to(dtype) for i in (3, 4))
+    w = 1 + 0.3 * torch.randn(dk, device="cuda", generator=gen(5))
+    buf, got = scratch(pk.pk_qk_norm_rope_bwd_scratch_bytes(T, Hq, Hkv, dk)), []
+    for a, b in ((torch.empty_like(q), torch.empty_like(k)), (q, k)):
+        dw = torch.zeros(2, dk, device="cuda")
+        pkt.check(pk.pk_qk_norm_rope_bwd(stream(), dt(q), ptr(gq), lq, ptr(gk), lk, ptr(q), lq, ptr(k), lk, ptr(w), ptr(w), ptr(a), lq, ptr(b), lk,
+                                         ptr(dw[0]), ptr(dw[1]), ptr(buf), T, Hq, Hkv, dk, 0, 0, 1e-6, None, None, 0))
+        got.append((a, b, dw))
+    assert all(torch.equal(x, y) for x, y in zip(*got))
