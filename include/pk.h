@@ -362,7 +362,7 @@ int pk_fill(void* stream, int dtype, void* dst, float value, int64_t n);
  * are not read, whatever they hold, nor is their target (-100 is usual); their outputs are 0. A word
  * masked with -inf or the type's lowest value has probability 0. A row that counts and holds NaN or
  * +inf, or nothing but -inf, gives NaN, as its softmax does. A row that counts and whose target
- * is out of range reports it and gives 0 and a zero gradient. Logits may start anywhere and have any
+ * is out of range reports it and gives 0 and a zero gradient. Logits may start at any element and have any
  * row stride >= V; every gradient is written to dlogits [R, V] (row stride ldd), which may be logits
  * itself (then ldd == ld); any other overlap is refused, and so are more than 2^28 - 1 rows.
  *

@@ -555,6 +555,7 @@ int pk_adamw_moment_unpack(void* stream, const void* codes, const uint8_t* scale
     PK_REQUIRE(n >= 0, "negative size");
     if (n == 0) return PK_OK;
     PK_REQUIRE(codes && scales && x, "null pointer");
+    PK_REQUIRE(aligned_to(4, x), "buffer not aligned to its type");
     const int64_t blocks = std::min<int64_t>((n + THREADS - 1) / THREADS, static_cast<int64_t>(sm_count()) * 16);
     moment_unpack_kernel<<<static_cast<unsigned>(blocks), THREADS, 0, as_stream(stream)>>>(
         static_cast<const uint8_t*>(codes), scales, x, n, root != 0);
@@ -566,6 +567,7 @@ int pk_adamw_moment_pack(void* stream, const float* x, void* codes, uint8_t* sca
     PK_REQUIRE(n >= 0, "negative size");
     if (n == 0) return PK_OK;
     PK_REQUIRE(x && codes && scales, "null pointer");
+    PK_REQUIRE(aligned_to(4, x), "buffer not aligned to its type");
     const int64_t blocks = std::min<int64_t>((n + THREADS - 1) / THREADS, static_cast<int64_t>(sm_count()) * 16);
     moment_pack_kernel<<<static_cast<unsigned>(blocks), THREADS, 0, as_stream(stream)>>>(
         x, static_cast<uint8_t*>(codes), scales, n, root != 0);

@@ -158,6 +158,11 @@ __host__ __device__ inline bool aligned16(const void* p) {
     return (reinterpret_cast<uintptr_t>(p) & 15u) == 0;
 }
 
+// Whether every given buffer (null: none) starts at a multiple of `size` bytes, as elements of that size must.
+template <typename... P> inline bool aligned_to(size_t size, const P*... p) {
+    return ((reinterpret_cast<uintptr_t>(p) | ...) & (size - 1)) == 0;
+}
+
 // ---- reductions ------------------------------------------------------------------
 __device__ __forceinline__ float warp_sum(float v) {
 #pragma unroll

@@ -561,6 +561,9 @@ int pk_qk_norm_rope_fwd(void* stream, int dtype, const void* q, int64_t ldq, con
     const bool turn = rot_q + rot_k > 0;
     PK_REQUIRE(!turn || (pos && cos_sin && n_pos > 0), "the rotation needs positions and a table");
     PK_REQUIRE((q != qo || ldq == ldqo) && (k != ko || ldk == ldko), "in place needs equal row strides");
+    PK_REQUIRE((Hq == 0 || aligned_to(dtype_size(dtype), q, qo)) && (Hkv == 0 || aligned_to(dtype_size(dtype), k, ko)) &&
+                   aligned_to(4, Hq ? wq : nullptr, Hkv ? wk : nullptr, turn ? pos : nullptr, turn ? cos_sin : nullptr),
+               "buffer not aligned to its type");
     {
         const size_t es = dtype_size(dtype);
         const Rows in[2] = {{q, ldq, cq}, {k, ldk, ck}}, out[2] = {{qo, ldqo, cq}, {ko, ldko, ck}};
@@ -610,6 +613,10 @@ int pk_qk_norm_rope_bwd(void* stream, int dtype, const void* dqo, int64_t lddqo,
     const bool gains = dwq != nullptr || dwk != nullptr;
     PK_REQUIRE(!gains || scratch, "the gains' gradients need scratch");
     PK_REQUIRE(!gains || dwq != dwk, "the two gains' gradients must be two buffers");
+    PK_REQUIRE((Hq == 0 || aligned_to(dtype_size(dtype), q, dqo, dq)) && (Hkv == 0 || aligned_to(dtype_size(dtype), k, dko, dk)) &&
+                   aligned_to(4, Hq ? wq : nullptr, Hkv ? wk : nullptr, dwq, dwk, turn ? pos : nullptr, turn ? cos_sin : nullptr) &&
+                   (!gains || aligned_to(4, static_cast<const char*>(scratch))),
+               "buffer not aligned to its type");
     {
         const size_t es = dtype_size(dtype);
         const Rows in[2] = {{q, ldq, cq}, {k, ldk, ck}}, up[2] = {{dqo, lddqo, cq}, {dko, lddko, ck}}, out[2] = {{dq, lddq, cq}, {dk, lddk, ck}};

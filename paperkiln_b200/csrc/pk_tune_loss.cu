@@ -707,6 +707,7 @@ int pk_token_logprob(void* stream, int dtype, const void* logits, int64_t ld, co
     PK_REQUIRE(R <= ROWS_MOST, "too many rows");
     if (R == 0) return PK_OK;
     PK_REQUIRE(logits && targets && logp && lse, "null pointer");
+    PK_REQUIRE(aligned_to(dtype_size(dtype), logits) && aligned_to(4, targets, weight, logp, lse, status), "buffer not aligned to its type");
     RowArgs a{};
     a.logits = logits; a.ld = ld; a.R = R; a.V = V; a.lse = lse;
     a.p.targets = targets; a.p.weight = weight; a.p.logp = logp; a.p.status = status;
@@ -720,6 +721,7 @@ int pk_token_logprob_bwd(void* stream, int dtype, const void* logits, int64_t ld
     PK_REQUIRE(R >= 0 && V > 0 && ld >= V && ldd >= V, "bad shape");
     if (R == 0) return PK_OK;
     PK_REQUIRE(logits && targets && lse && dlogp && dlogits, "null pointer");
+    PK_REQUIRE(aligned_to(dtype_size(dtype), logits, dlogits) && aligned_to(4, targets, lse, dlogp, status), "buffer not aligned to its type");
     PK_REQUIRE(!bad_alias(logits, ld, dlogits, ldd, R, V, dtype_size(dtype)), "dlogits overlaps logits");
     const int threads = row_threads(V);
     // few rows: several blocks to a row, down to two vectors per thread (80 rows of 32000 bf16: 9.7 -> 7.0 us)
@@ -739,6 +741,7 @@ int pk_preference_loss(void* stream, const float* logp, const float* ref_logp, c
     PK_REQUIRE(label_smoothing >= 0.0f && label_smoothing <= 1.0f, "label_smoothing must be in [0, 1]");
     if (n_pairs == 0) return PK_OK;
     PK_REQUIRE(seq && loss && (R == 0 || logp), "null pointer");
+    PK_REQUIRE(aligned_to(4, logp, ref_logp, weight, seq, loss, margin, dlogp, status), "buffer not aligned to its type");
     return launch(as_stream(stream), preference_loss_kernel, dim3(static_cast<unsigned>(n_pairs)), 1, PAIR_THREADS, logp, ref_logp, weight, seq,
                   R, beta, label_smoothing, grad_scale, loss, margin, dlogp, status);
 }
@@ -753,6 +756,9 @@ int pk_policy_loss(void* stream, int dtype, const void* logits, int64_t ld, cons
     PK_REQUIRE(clip_lo >= 0.0f && clip_lo <= 1.0f && clip_hi >= 0.0f, "clip bounds must not be negative, the lower at most 1");
     if (R == 0) return PK_OK;
     PK_REQUIRE(logits && targets && advantage && row_loss, "null pointer");
+    PK_REQUIRE(aligned_to(dtype_size(dtype), logits, dlogits) &&
+                   aligned_to(4, targets, old_logp, ref_logp, advantage, weight, row_loss, logp, kl, status),
+               "buffer not aligned to its type");
     PK_REQUIRE(!bad_alias(logits, ld, dlogits, ldd, R, V, dtype_size(dtype)), "dlogits overlaps logits");
     const PolicyArgs a = {targets, old_logp, ref_logp, advantage, weight, 1.0f - clip_lo, 1.0f + clip_hi, kl_coef, grad_scale,
                           row_loss, logp, kl, status};

@@ -248,3 +248,35 @@ def test_head_norm_gradients_refuse_outputs_inside_their_inputs(pk, size):
     assert f(dq=(4 * BASE, 0, 64)) and f(dk_=at["dqo"]) and f(dk_=at["q"]) and f(dk_=(FAR, 0, 64))
     packed = {"dqo": (BASE, 0, 160), "dko": (BASE, 64, 160), "dq": (BASE, 0, 160), "dk_": (BASE, 64, 160)}
     assert not f(**packed) and not f(**(packed | {"dk_": (BASE, 96, 160)})) and f(**(packed | {"dk_": (BASE, 60, 160)}))
+
+
+# ---- addresses that no element of the type can have --------------------------------------------
+
+@pytest.mark.skipif(torch.cuda.is_available(), reason="names addresses without memory")
+def test_buffers_off_their_type_are_refused(pk):
+    """Rows may start at any element, but not between two bytes of one: the kernels' loads would fault."""
+    P = [ctypes.c_void_p((i + 1) << 26) for i in range(20)]
+    odd = lambda p, n: ctypes.c_void_p(p.value + n)  # noqa: E731
+
+    def each(call, args, sizes):
+        """call(*args) gets as far as the GPU; with any one buffer (sizes: {index: bytes of an element}) moved it is refused."""
+        assert call(*args) == 2
+        for i, size in sizes.items():
+            for off in (1, 2) if size == 4 else (1,):
+                moved = list(args)
+                moved[i] = odd(args[i], off)
+                assert call(*moved) == 1 and b"aligned" in pk.pk_last_error(), (i, off)
+
+    for dtype, es in ((0, 4), (1, 2)):
+        each(pk.pk_token_logprob, [None, dtype, P[0], 8, P[1], P[2], P[3], P[4], 2, 8, P[5]], {2: es, 4: 4, 5: 4, 6: 4, 7: 4, 10: 4})
+        each(pk.pk_token_logprob_bwd, [None, dtype, P[0], 8, P[1], P[2], P[3], P[4], 8, 2, 8, P[5]], {2: es, 4: 4, 5: 4, 6: 4, 7: es, 11: 4})
+        each(pk.pk_policy_loss, [None, dtype, P[0], 8, P[1], P[2], P[3], P[4], P[5], 0.2, 0.2, 0.1, 1.0, P[6], P[7], P[8], P[9], 8, 2, 8, P[10]],
+             {2: es, 4: 4, 5: 4, 6: 4, 7: 4, 8: 4, 13: 4, 14: 4, 15: 4, 16: es, 20: 4})
+        each(pk.pk_qk_norm_rope_fwd, [None, dtype, P[0], 64, P[1], 32, P[2], P[3], P[4], 64, P[5], 32, 3, 4, 2, 16, 4, 2, 1e-6, P[6], P[7], 8],
+             {2: es, 4: es, 6: 4, 7: 4, 8: es, 10: es, 19: 4, 20: 4})
+        each(pk.pk_qk_norm_rope_bwd, [None, dtype, P[0], 64, P[1], 32, P[2], 64, P[3], 32, P[4], P[5], P[6], 64, P[7], 32, P[8], P[9], P[10], 3, 4, 2, 16,
+                                      4, 2, 1e-6, P[11], P[12], 8],
+             {2: es, 4: es, 6: es, 8: es, 10: 4, 11: 4, 12: es, 14: es, 16: 4, 17: 4, 18: 4, 26: 4, 27: 4})
+    each(pk.pk_preference_loss, [None, P[0], P[1], P[2], P[3], 1, 4, 0.1, 0.0, 1.0, P[4], P[5], P[6], P[7]], {1: 4, 2: 4, 3: 4, 4: 4, 10: 4, 11: 4, 12: 4, 13: 4})
+    each(pk.pk_adamw_moment_unpack, [None, P[0], P[1], P[2], 4, 0], {3: 4})
+    each(pk.pk_adamw_moment_pack, [None, P[0], P[1], P[2], 4, 0], {1: 4})
