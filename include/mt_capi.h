@@ -106,7 +106,8 @@ int mt_model_set_adamw(void* model, float lr, float beta1, float beta2, float ep
 int mt_model_optimizer_step(void* model);
 /* Bits of the stored moments, 32 (default) or 8 (2.06 bytes per parameter instead of 8, see pk_adamw_multi);
  * before the first step. mt_model_save / load and the state entries below keep working: the moments are
- * converted to fp32 and back without loss, and a restored run continues bit-identically. */
+ * converted to fp32 and back without loss as long as no stored sqrt(v) above zero is below 2^-71 (v below 2^-142: its
+ * square has no exact fp32) or at 2^64 and above, and a restored run then continues bit-identically. */
 int mt_model_set_adamw_state_bits(void* model, int bits);
 /* Learning-rate factor and weight decay of one parameter (index of mt_model_param_info) from the next step on;
  * the others keep (1, the decay of mt_model_set_adamw). */

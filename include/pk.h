@@ -450,7 +450,8 @@ int pk_adamw_multi(void* stream, void* plan_h, float lr, float b1, float b2, flo
 /* 8-bit moments to fp32 and back, for checkpoints: x = code * 2^(byte - 127), and codes and scales of x
  * with every value rounded to nearest (root = 0, the form of m) or to nearest with nothing above zero
  * becoming zero (root = 1, the form of sqrt(v): the entries then convert v itself, squaring and taking the
- * root). */
+ * root). Packing what was unpacked gives the same values; with root = 1 as long as every stored root is 0 or in
+ * [2^-71, 2^64), outside of which its square is rounded, becomes 0 or infinite in fp32. */
 int pk_adamw_moment_unpack(void* stream, const void* codes, const uint8_t* scales, float* x, int64_t n, int root);
 int pk_adamw_moment_pack(void* stream, const float* x, void* codes, uint8_t* scales, int64_t n, int root);
 /* Q8_0: blocks of 32 along a row of W[rows, cols] (cols % 32 == 0), int8 values and an

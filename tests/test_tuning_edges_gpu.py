@@ -248,3 +248,19 @@ def test_head_norm_gradients_over_the_inputs(pk, dtype, shape):  # noqa: F811
                                          ptr(dw[0]), ptr(dw[1]), ptr(buf), T, Hq, Hkv, dk, 0, 0, 1e-6, None, None, 0))
         got.append((a, b, dw))
     assert all(torch.equal(x, y) for x, y in zip(*got))
+
+
+@pytest.mark.parametrize("root, first, last", [(0, 1, 246), (1, 65, 182)])
+def test_every_stored_moment_survives_fp32(pk, root, first, last):  # noqa: F811
+    """All codes under all scales through fp32 and back: the same values. For roots the scales whose smallest code is
+    2^-71 and whose largest is below 2^64."""
+    codes = torch.arange(128, device="cuda", dtype=torch.uint8) % 127   # no NaN
+    scales = torch.arange(first, last + 1, device="cuda", dtype=torch.uint8)
+    c, b = codes.repeat(scales.numel()), scales.repeat_interleave(4)
+    if not root:
+        c = c | (torch.arange(c.numel(), device="cuda") % 3 == 0).to(torch.uint8) * 128
+    n = c.numel()
+    x, c2, b2 = torch.empty(n, device="cuda"), torch.empty_like(c), torch.empty_like(b)
+    pkt.check(pk.pk_adamw_moment_unpack(stream(), ptr(c), ptr(b), ptr(x), n, root))
+    pkt.check(pk.pk_adamw_moment_pack(stream(), ptr(x), ptr(c2), ptr(b2), n, root))
+    assert torch.equal(ops.decode(c2, b2), ops.decode(c, b))
