@@ -38,8 +38,9 @@ Var linear_cross_entropy(const Var& h, const Var& W, bool transposed_w, const st
 // ---- preference / policy tuning (no counterpart in the reference) -------------------------------
 // The losses of pk_policy_loss and pk_preference_loss over the rows of h W (or h W^T), chunked like
 // linear_cross_entropy. Empty vectors leave a term out; rows of weight 0 do not count, whatever their
-// target. The policy loss is the SUM of the weighted row losses (the caller's weights normalise it); the
-// preference loss is the mean over the pairs. *logp, *kl, *pair_loss, *margin (may be null) receive host copies.
+// target, nor do rows of no sequence in the preference loss. The policy loss is the SUM of the weighted row
+// losses (the caller's weights normalise it); the preference loss is the mean over the pairs. *logp, *kl,
+// *pair_loss, *margin (may be null) receive host copies.
 struct PolicyTerms {
     std::vector<float> old_logp, ref_logp, advantage, weight;
     float clip_lo = 0.2f, clip_hi = 0.2f, kl_coef = 0.0f;

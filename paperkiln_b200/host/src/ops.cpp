@@ -1015,14 +1015,21 @@ Var linear_preference_loss(const Var& h, const Var& W, bool transposed_w, const 
                            size_t chunk_rows, std::vector<float>* loss_out, std::vector<float>* margin_out) {
     HeadChunks head(h, W, transposed_w, chunk_rows);
     const size_t R = head.R;
-    check_targets(targets, terms.weight, R, head.V);
     if (terms.seq.size() < 3 || terms.seq.size() % 2 == 0) throw std::runtime_error("preference_loss: 2 n + 1 offsets for n pairs");
     for (size_t i = 0; i < terms.seq.size(); ++i)
         if (terms.seq[i] < (i ? terms.seq[i - 1] : 0) || static_cast<size_t>(terms.seq[i]) > R)
             throw std::runtime_error("preference_loss: offsets must ascend within the rows");
+    std::vector<float> counts = terms.weight;
+    const size_t first = static_cast<size_t>(terms.seq.front()), last = static_cast<size_t>(terms.seq.back());
+    if (first > 0 || last < R) {  // rows outside every sequence do not count, whatever their targets
+        if (counts.empty()) counts.assign(R, 1.0f);
+        for (size_t i = 0; i < counts.size(); ++i)
+            if (i < first || i >= last) counts[i] = 0.0f;
+    }
+    check_targets(targets, counts, R, head.V);
     const size_t P = terms.seq.size() / 2;
     Tensor dtg = device_ints(targets), seq = device_ints(terms.seq);
-    Tensor ref = row_values(terms.ref_logp, R, "preference_loss"), weight = row_values(terms.weight, R, "preference_loss");
+    Tensor ref = row_values(terms.ref_logp, R, "preference_loss"), weight = row_values(counts, R, "preference_loss");
     Tensor logp = Tensor::empty(1, R, DType::F32), lse = Tensor::empty(1, R, DType::F32);
     Tensor dlogp = Tensor::zeros(1, R, DType::F32);  // rows outside every sequence keep a gradient of zero
     Tensor pair = Tensor::empty(1, P, DType::F32), margin = Tensor::empty(1, P, DType::F32);
