@@ -3,7 +3,8 @@
 // The plan is a table of chunks in device memory, one CTA each. Per element the step reads p, g and both
 // moments and writes p, both moments and the bf16 shadow: 30 bytes with fp32 moments and gradients, 18.1 with
 // 8-bit moments. Bound by memory: 124 M parameters with fp32 moments 535 us, as fast as a copy; 243 M with 8-bit
-// moments 811 us, 5.4 TB/s (84 % of a copy), where the coding of the moments shares the issue slots.
+// moments 795 - 815 us from card to card, 5.4 TB/s (85 % of a copy), where the coding of the moments shares the
+// issue slots.
 //
 // 8-bit moments: E4M3 codes, one power-of-two scale per 32 elements. A scale that is a power of two
 // makes both directions exact but for the rounding of the code itself. sqrt(v) is stored instead

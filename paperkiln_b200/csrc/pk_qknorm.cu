@@ -8,7 +8,8 @@
 // nothing saved by the forward and reduces once.
 //
 // Bound by memory: 2 (forward) or 3 (backward) accesses per element. bf16: 65536 x 40 heads of 64 take
-// 120 us forward, 5.6 TB/s; 16381 x 32 heads of 128 take 76 us backward, 5.3 TB/s, the sum of dw included.
+// 118 - 124 us forward from card to card, 5.6 TB/s; 16381 x 32 heads of 128 73 - 75 us backward, 5.5 TB/s, the sum
+// of dw included.
 // A team of LANES threads owns a head, 16 bytes per thread. A warp's task is a group of heads of one kind
 // and one token (of several tokens where a token has fewer heads than the warp has teams): U heads per
 // team, all loaded before the first is computed, with the rotation table's row and the gains in registers.
@@ -23,8 +24,8 @@ namespace pk {
 namespace {
 
 constexpr int THREADS = 256, WARPS = THREADS / 32;  // of the backward
-// Small CTAs in the forward, nine to an SM at 56 registers (65536 x 40 heads of 64: 120 us; four of 256 at 64
-// registers 130, ten at 48 120, and 118 against 114 at head_dim 128).
+// Small CTAs in the forward, nine to an SM at 56 registers (65536 x 40 heads of 64, on one card: 120 us; four of 256 at
+// 64 registers 130, ten at 48 120, and 118 against 114 at head_dim 128).
 constexpr int FWD_THREADS = 128, FWD_WARPS = FWD_THREADS / 32;
 constexpr int U = 4;  // heads per team in flight, at most
 

@@ -27,8 +27,9 @@ __device__ __forceinline__ float ex2(float x) {
 
 // The kernels of this file are launched while their predecessor on the stream still runs, and wait for it here
 // before they touch memory: the cost of a launch is then behind them. None of their parameters is __restrict__: that
-// would allow loads that are defined only for data that nobody writes while the kernel lives, and the predecessor does. The three calls of a paired loss, 2 x 40 rows of
-// 32000 bf16: 21 -> 16 us, 8192 rows 210 -> 204; replayed from a graph, where a launch costs little, 9.4 -> 10.6.
+// would allow loads that are defined only for data that nobody writes while the kernel lives, and the predecessor does.
+// The three calls of a paired loss over 32000 words in bf16, 8192 rows: 224 -> 218 us; 2 x 40 rows, called from Python,
+// 25 -> 23, and replayed from a graph, where a launch costs little, 9.6 -> 10.7.
 __device__ __forceinline__ void after_predecessor() {
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -355,11 +356,13 @@ __device__ __forceinline__ uint4 pack(const float (&f)[8]) {
 // logits once. Nothing orders the rows: the chain from a row's last byte over its reductions to its scalars is
 // hidden by what else is resident.
 //
-// Bound by memory and its latency. Policy loss with its gradient, bf16: 8192 x 32000 189 us, 5.5 TB/s (second
-// reading forwards 195), 60000 x 4000 168 us, 5.7 TB/s, 8192 x 151936 928 us, 5.4 TB/s. A row that stays in the
-// registers or the shared memory of its CTAs while the next one is on its way with cp.async took 207 at the first size
-// and 385 at the second: its warps wait for one another between the rows. Holding a part of the stretch in
-// shared memory for the second reading costs L1 as much as it saves (190; five CTAs per SM). Without a gradient:
+// Bound by memory and its latency. Policy loss with its gradient, bf16: 8192 x 32000 185 - 189 us from card to card, 5.6
+// TB/s (second reading forwards 195), 60000 x 4000 168 us, 5.7 TB/s, 8192 x 151936 930 - 1010 us, 5.2 TB/s, where the
+// second reading is no cause: DRAM moves 931 MB of the 934 that 1536 such rows and their gradient have, and 833 of 817
+// with a quarter of dead rows. A row that stays in the registers or the shared memory of its CTAs while the next one is
+// on its way with cp.async took 207 at the first size and 385 at the second (kept: 189 and 168 on that card): its warps
+// wait for one another between the rows. Holding a part of the stretch in shared memory for the second reading costs
+// L1 as much as it saves (190; five CTAs per SM). Without a gradient:
 // 8192 x 50257 150 us, 5.5 TB/s.
 constexpr int CLUSTER_MOST = 8, SWEEP_K = 4;
 constexpr int64_t ROWS_MOST = 0x7fffffff / CLUSTER_MOST;  // of a call with one grid for all rows
