@@ -218,7 +218,7 @@ int pk_gemm_rope(void* stream, int trans_b, int64_t M, int64_t N, int64_t K, con
  * may be NULL. Norm and rotation are fp32, the result is rounded once. Outputs may be the inputs
  * themselves (same pointer and stride: in place); any other overlap is refused (column ranges of one buffer are apart when
  * they are within the row stride, with two strides within the greatest common divisor of both). Any even
- * head_dim up to 256, any strides and alignment (16-byte aligned rows take wide accesses).
+ * head_dim up to 256, any strides, rows from any element on (16-byte aligned ones take wide accesses).
  * The backward takes the upstream gradients dqo / dko and the inputs q / k of the forward (nothing
  * else is saved: the norm is recomputed from the row it reads anyway) and writes dq / dk, which may
  * be dqo / dko or q / k; dwq and dwk are ACCUMULATED (+=), each may be NULL. Replaces ops::rmsnorm per head
